@@ -75,8 +75,9 @@ LALB_API int         lalb_destroy(lalb_ctx *ctx);
 /* Text of the last error recorded on this context ("" if none). */
 LALB_API const char *lalb_last_error(const lalb_ctx *ctx);
 /* Synchronises the device and returns the device-side status word, a set
- * of bits: 1 = a bounded wait expired, 2 = a decode position outside the KV
- * cache was refused (0 = neither); reset != 0 clears it. */
+ * of bits: 1 = a bounded wait expired, 2 = a decode position, a slot or a
+ * length outside the KV cache was refused (0 = neither); reset != 0 clears
+ * it. */
 LALB_API int         lalb_device_status(lalb_ctx *ctx, int reset);
 
 /* ---- formats ---------------------------------------------------------- */
@@ -161,6 +162,107 @@ LALB_API int lalb_attention_decode(lalb_ctx *ctx, const float *qkv, int n_head, 
                                    int head_dim, int pos, int max_ctx, float rope_theta,
                                    float *k_cache, float *v_cache, float *out,
                                    lalb_stream stream);
+
+/* ---- a batch of sequences: cache, rotary append, attention, eviction -----
+ * The KV cache of one layer for n_seq sequences.  Sequence b holds rows
+ * b*max_ctx .. of k and v; a row is n_kv_head*head_dim values.  row_pos and
+ * row_weight (both nullable) hold, per sequence and KV head, each row's
+ * position and the attention weight it has gathered ([n_seq][n_kv_head]
+ * [max_ctx]): eviction keeps different rows for each KV head, so a row's
+ * position is known per head.  Rows may be in any order (their keys are
+ * already rotated).  All buffers are device memory of the caller; k and v
+ * 16-byte aligned.  head_dim 32, 64, 128 or 256; n_seq*max_ctx < 2^31. */
+typedef struct {
+    int dtype;               /* LALB_DT_F32, LALB_DT_F16 or LALB_DT_BF16 */
+    int n_seq, max_ctx, n_kv_head, head_dim;
+    void *k, *v;             /* [n_seq][max_ctx][n_kv_head*head_dim] */
+    int32_t *row_pos;        /* [n_seq][n_kv_head][max_ctx], nullable */
+    float *row_weight;       /* [n_seq][n_kv_head][max_ctx], nullable */
+} lalb_kv_batch;
+
+/* Rotary positions.  Pair d of the rot_dim/2 rotated pairs turns by
+ * pos * f_d, f_d = theta^(-2d/rot_dim):
+ *   layout  HALF pairs elements (d, d + rot_dim/2), INTERLEAVED (2d, 2d+1);
+ *           elements rot_dim.. of a head pass unrotated;
+ *   scaling LINEAR divides f_d by factor; PARTS keeps the pairs that turn
+ *           often within the original context and divides those that do not:
+ *           t = orig_ctx f_d / 2 pi turns, g = clamp((t - turns_slow) /
+ *           (turns_fast - turns_slow), 0, 1), f_d (g + (1 - g) / factor);
+ *   mscale  multiplies cos and sin.
+ * Zero selects a default: rot_dim head_dim, theta 10000, mscale 1.  rot_dim
+ * a multiple of 8.  Angles are reduced in double, the rotation is fp32. */
+enum { LALB_ROPE_HALF = 0, LALB_ROPE_INTERLEAVED = 1 };
+enum { LALB_ROPE_UNSCALED = 0, LALB_ROPE_LINEAR = 1, LALB_ROPE_PARTS = 2 };
+typedef struct {
+    int layout;
+    int rot_dim;
+    float theta;
+    int scaling;
+    float factor, orig_ctx, turns_fast, turns_slow;
+    float mscale;
+} lalb_rope;
+
+/* T tokens enter the cache (apply_rope, runtime/lal_runtime.c:137-153, for a
+ * batch of tokens of any sequences).  Token t is row t of qkv, qkv_stride
+ * elements apart: q [n_head*head_dim] | k | v [n_kv_head*head_dim each], of
+ * type qkv_dtype (LALB_DT_F32 or the cache's type).  Its q rotated to
+ * positions[t] goes to row t of q_out ([T][n_head*head_dim], the cache's
+ * type); its rotated k and its v go to cache row slots[t] = b*max_ctx + j,
+ * with row_pos[b][.][j] = positions[t] and row_weight[b][.][j] = 0 where
+ * those are given.  slots[t] < 0 (padding) stores nothing; a slot past the
+ * cache stores nothing and raises status bit 2 (lalb_device_status).  No two
+ * tokens of a call may have the same slot.  slots NULL: only q is rotated.
+ * A negative position turns back, so that a rotation's gradient is the
+ * rotation by the negated positions.  qkv rows and q_out 16-byte aligned. */
+LALB_API int lalb_rope_append(lalb_ctx *ctx, const lalb_rope *rope, const lalb_kv_batch *cache,
+                              int n_head, const void *qkv, int qkv_dtype, long long qkv_stride,
+                              int T, const int32_t *positions, const int32_t *slots, void *q_out,
+                              lalb_stream stream);
+
+/* One query token per sequence: q row b attends the prefix_len rows of
+ * prefix_k / prefix_v ([prefix_len][n_kv_head*head_dim] of the cache's type,
+ * shared by every sequence and read once for all of them) and the first
+ * lens[b] rows of its own cache (0 <= lens[b] <= max_ctx, on the device):
+ * out [n_seq][n_head*head_dim] = softmax(scale q k) v over both, head h on KV
+ * head h / (n_head / n_kv_head), 0 for a sequence with no rows at all.  scale
+ * 0 selects 1/sqrt(head_dim).  With add_weights, row_weight[b][g][j] =
+ * decay * row_weight[b][g][j] + the softmax weights of row j summed over the
+ * q heads of KV head g, for j < lens[b] (decay 0: the old value is not
+ * read); the prefix rows' weights are not kept.  q, the caches and out have
+ * the cache's type; q row b starts at q + b*q_stride elements.  A
+ * length outside its range counts as 0 and raises status bit 2.  ws: from
+ * lalb_attention_batch_ws_bytes, 256-byte aligned, nothing kept between
+ * calls; calls that may overlap need one each.  The result does not depend
+ * on scheduling. */
+typedef struct {
+    int n_head;
+    float scale;
+    int prefix_len;
+    const void *prefix_k, *prefix_v;   /* NULL with prefix_len 0 */
+    int add_weights;
+    float decay;
+} lalb_attn_batch;
+LALB_API int lalb_attention_batch_ws_bytes(const lalb_kv_batch *cache, const lalb_attn_batch *attn,
+                                           size_t *bytes);
+LALB_API int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache,
+                                  const lalb_attn_batch *attn, const void *q, long long q_stride,
+                                  const int32_t *lens, void *ws, void *out, lalb_stream stream);
+
+/* Cuts every sequence with more than `keep` rows down to `keep`, for each KV
+ * head by itself.  Kept are the rows at a position below n_sink, those among
+ * the last n_recent positions (above the largest row_pos - n_recent), then
+ * the rows of the largest row_weight (a NaN ranks lowest), ties to the lower
+ * row.  Kept rows below `keep` stay where they are; the i-th kept row above
+ * moves into the i-th row given up below, so that only those rows are
+ * copied.  Afterwards lens[b] = keep and row_weight of rows keep..old
+ * length-1 is 0; the rest of those rows, and all rows behind them, are left as
+ * they were.  Sequences of at most `keep` rows are left as they are; a length
+ * outside [0, max_ctx] raises status bit 2 and is left too.  The cache needs row_pos and row_weight.
+ * 1 <= keep <= max_ctx, n_sink + n_recent <= keep.  ws: from
+ * lalb_kv_evict_ws_bytes, 256-byte aligned. */
+LALB_API int lalb_kv_evict_ws_bytes(const lalb_kv_batch *cache, int keep, size_t *bytes);
+LALB_API int lalb_kv_evict(lalb_ctx *ctx, const lalb_kv_batch *cache, int32_t *lens, int keep,
+                           int n_sink, int n_recent, void *ws, lalb_stream stream);
 
 /* ---- next-token sampling after the LM head --------------------------------
  * generate_text's sampling (models/ste_train.c:2229-2318) on device logits:

@@ -26,7 +26,7 @@ QK_K = 256
 QB = 32
 Q4K_BLOCK_BYTES = 144
 
-__all__ = ["Context", "Decoder", "LalbError", "lal_matmul_q4_k", "lal_lm_head_int8_range",
+__all__ = ["Context", "Decoder", "KVBatch", "Rope", "LalbError", "lal_matmul_q4_k", "lal_lm_head_int8_range",
            "unpack_scales_6bit", "q4k_row_bytes", "QK_K", "QB", "Q4K_BLOCK_BYTES"]
 
 
@@ -40,6 +40,26 @@ def _p(t):
 
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _want(who, name, t, device, dtype, numel=None, optional=False):
+    """Checks of a tensor whose address goes to the library."""
+    if t is None and optional:
+        return
+    ok = (isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype and t.is_contiguous()
+          and (numel is None or t.numel() == numel))
+    if not ok:
+        raise LalbError(who, -1, "%s must be a contiguous %s tensor%s on %s" %
+                        (name, dtype, "" if numel is None else " of %d elements" % numel, device))
+
+
+def _want_rows(who, name, t, device, dtype, rows, cols):
+    """Checks of a matrix whose rows may lie apart; returns their distance."""
+    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype and t.dim() == 2
+            and tuple(t.shape) == (rows, cols) and t.stride(1) == 1 and (rows < 2 or t.stride(0) >= cols)):
+        raise LalbError(who, -1, "%s must be a %s matrix [%d][%d] with contiguous rows on %s" %
+                        (name, dtype, rows, cols, device))
+    return t.stride(0) if rows > 1 else cols
 
 
 def unpack_scales_6bit(scales12):
@@ -145,6 +165,111 @@ class Context:
                    _stream())
         return out
 
+    # ---- a batch of sequences -----------------------------------------------
+    def _batch_stream(self):
+        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def rope_append(self, cache, qkv, positions, slots, n_head, rope=None, out=None):
+        """T tokens enter a KVBatch (lalb_rope_append): qkv [T][(n_head + 2
+        n_kv_head) * head_dim] (float32 or the cache's type; rows may lie
+        apart), positions int32 [T], slots int32 [T] (cache row b * max_ctx +
+        j, negative: padding) or None to rotate q alone.  Writes the rotated k
+        and the v to their rows and returns the rotated q [T][n_head *
+        head_dim] in the cache's type."""
+        who = "lalb_rope_append"
+        T = qkv.shape[0]
+        hd, width = cache.head_dim, n_head * cache.head_dim
+        cols = width + (0 if slots is None else 2 * cache.n_kv_head * hd)
+        cache.check(who, self.device)
+        if qkv.dtype not in (torch.float32, cache.k.dtype):
+            raise LalbError(who, -1, "qkv must be float32 or of the cache's type")
+        stride = _want_rows(who, "qkv", qkv, self.device, qkv.dtype, T, cols)
+        _want(who, "positions", positions, self.device, torch.int32, T)
+        _want(who, "slots", slots, self.device, torch.int32, T, optional=True)
+        if out is None:
+            out = torch.empty((T, width), dtype=cache.k.dtype, device=self.device)
+        _want(who, "out", out, self.device, cache.k.dtype, T * width)
+        if T == 0:
+            return out
+        self._call(who, self.h, ctypes.byref((rope or Rope()).desc), ctypes.byref(cache.desc), n_head, _p(qkv),
+                   _DT[qkv.dtype], stride, T, _p(positions), _p(slots), _p(out), self._batch_stream())
+        return out
+
+    def attention_batch_ws(self, cache, n_head, prefix_len=0, weights=False):
+        """Workspace of attention_batch calls with a prefix of prefix_len rows
+        at most."""
+        a = _abi.AttnBatchDesc(n_head, 0.0, prefix_len, None, None, int(weights), 0.0)
+        return self._batch_ws("lalb_attention_batch_ws_bytes", ctypes.byref(cache.desc), ctypes.byref(a))
+
+    def _batch_ws(self, name, *args):
+        n = ctypes.c_size_t()
+        st = getattr(_abi.lib(), name)(*args, ctypes.byref(n))
+        if st:
+            raise LalbError(name, st)
+        return torch.empty(n.value, dtype=torch.uint8, device=self.device)
+
+    def attention_batch(self, cache, q, lens, n_head, prefix_k=None, prefix_v=None, scale=0.0, decay=None,
+                        ws=None, out=None):
+        """One query token per sequence over a shared prefix and the sequence's
+        own rows (lalb_attention_batch): q [n_seq][n_head * head_dim] of the
+        cache's type (rows may lie apart), lens int32 [n_seq], prefix_k /
+        prefix_v [prefix_len][n_kv_head * head_dim] or None.  decay given: the
+        cache's row_weight = decay * row_weight + this step's weights.
+        Returns out [n_seq][n_head * head_dim]."""
+        who = "lalb_attention_batch"
+        cache.check(who, self.device)
+        width, kvr, dt = n_head * cache.head_dim, cache.n_kv_head * cache.head_dim, cache.k.dtype
+        stride = _want_rows(who, "q", q, self.device, dt, cache.n_seq, width)
+        _want(who, "lens", lens, self.device, torch.int32, cache.n_seq)
+        prefix = 0
+        if (prefix_k is None) != (prefix_v is None):
+            raise LalbError(who, -1, "prefix_k and prefix_v come together")
+        if prefix_k is not None:
+            prefix = prefix_k.numel() // kvr
+            _want(who, "prefix_k", prefix_k, self.device, dt, prefix * kvr)
+            _want(who, "prefix_v", prefix_v, self.device, dt, prefix * kvr)
+        a = _abi.AttnBatchDesc(n_head, scale, prefix, _p(prefix_k) if prefix else None,
+                               _p(prefix_v) if prefix else None, int(decay is not None), decay or 0.0)
+        n = ctypes.c_size_t()
+        st = _abi.lib().lalb_attention_batch_ws_bytes(ctypes.byref(cache.desc), ctypes.byref(a), ctypes.byref(n))
+        if st:
+            raise LalbError("lalb_attention_batch_ws_bytes", st)
+        if ws is None:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
+        _want(who, "ws", ws, self.device, torch.uint8)
+        if ws.numel() < n.value:
+            raise LalbError(who, -1, "ws holds %d bytes of %d" % (ws.numel(), n.value))
+        if out is None:
+            out = torch.empty((cache.n_seq, width), dtype=dt, device=self.device)
+        _want(who, "out", out, self.device, dt, cache.n_seq * width)
+        self._call(who, self.h, ctypes.byref(cache.desc), ctypes.byref(a), _p(q), stride, _p(lens), _p(ws), _p(out),
+                   self._batch_stream())
+        return out
+
+    def kv_evict_ws(self, cache, keep):
+        """Workspace of kv_evict calls that keep `keep` rows."""
+        return self._batch_ws("lalb_kv_evict_ws_bytes", ctypes.byref(cache.desc), keep)
+
+    def kv_evict(self, cache, lens, keep, n_sink=0, n_recent=0, ws=None):
+        """Cuts every sequence of a KVBatch to the `keep` rows that matter
+        (lalb_kv_evict): the first n_sink positions, the last n_recent, then
+        the largest row_weight.  Updates the cache, its row_pos and row_weight
+        and lens (int32 [n_seq])."""
+        who = "lalb_kv_evict"
+        cache.check(who, self.device)
+        _want(who, "lens", lens, self.device, torch.int32, cache.n_seq)
+        n = ctypes.c_size_t()
+        st = _abi.lib().lalb_kv_evict_ws_bytes(ctypes.byref(cache.desc), keep, ctypes.byref(n))
+        if st:
+            raise LalbError("lalb_kv_evict_ws_bytes", st, "keep %d" % keep)
+        if ws is None:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
+        _want(who, "ws", ws, self.device, torch.uint8)
+        if ws.numel() < n.value:
+            raise LalbError(who, -1, "ws holds %d bytes of %d" % (ws.numel(), n.value))
+        self._call(who, self.h, ctypes.byref(cache.desc), _p(lens), keep, n_sink, n_recent, _p(ws),
+                   self._batch_stream())
+
     def sample(self, logits, history=None, temperature=0.0, top_k=1, top_p=0.9,
                rep_penalty=1.0, no_repeat_ngram=0, n_masked_low_ids=0, u=None, want_topk=False):
         """Next token from device logits (lalb_sample).  history: int32 CUDA
@@ -197,6 +322,49 @@ class Context:
 
 
 MMA_F16, MMA_I8 = 0, 1   # LALB_MMA_F16, LALB_MMA_I8
+
+_DT = {torch.float32: 0, torch.float16: 3, torch.bfloat16: 4}   # LALB_DT_F32, _F16, _BF16
+
+
+class KVBatch:
+    """One layer's KV cache for a batch of sequences (include/lalb.h,
+    lalb_kv_batch): k, v CUDA tensors [n_seq][max_ctx][n_kv_head * head_dim]
+    (float32, float16 or bfloat16); row_pos int32 and row_weight float32
+    [n_seq][n_kv_head][max_ctx], both optional."""
+
+    def __init__(self, k, v, n_kv_head, row_pos=None, row_weight=None):
+        if k.dim() != 3 or k.dtype not in _DT or n_kv_head < 1 or k.shape[2] % n_kv_head:
+            raise LalbError("KVBatch", -1, "k must be a float32, float16 or bfloat16 tensor "
+                                           "[n_seq][max_ctx][n_kv_head * head_dim]")
+        self.k, self.v, self.row_pos, self.row_weight = k, v, row_pos, row_weight
+        self.n_seq, self.max_ctx = k.shape[0], k.shape[1]
+        self.n_kv_head, self.head_dim = n_kv_head, k.shape[2] // n_kv_head
+        self.check("KVBatch", k.device)
+        self.desc = _abi.KVBatchDesc(_DT[k.dtype], self.n_seq, self.max_ctx, n_kv_head, self.head_dim, _p(k), _p(v),
+                                     _p(row_pos), _p(row_weight))
+
+    def check(self, who, device):
+        rows = self.n_seq * self.n_kv_head * self.max_ctx
+        _want(who, "k", self.k, device, self.k.dtype)
+        _want(who, "v", self.v, device, self.k.dtype, self.k.numel())
+        _want(who, "row_pos", self.row_pos, device, torch.int32, rows, optional=True)
+        _want(who, "row_weight", self.row_weight, device, torch.float32, rows, optional=True)
+
+
+class Rope:
+    """Rotary parameters (include/lalb.h, lalb_rope).  layout "half" or
+    "interleaved"; rot_dim 0: the whole head; scaling "none", "linear" or
+    "parts"."""
+
+    LAYOUTS = {"half": 0, "interleaved": 1}
+    SCALINGS = {"none": 0, "linear": 1, "parts": 2}
+
+    def __init__(self, layout="half", rot_dim=0, theta=0.0, scaling="none", factor=1.0, orig_ctx=0.0,
+                 turns_fast=32.0, turns_slow=1.0, mscale=0.0):
+        if layout not in self.LAYOUTS or scaling not in self.SCALINGS:
+            raise LalbError("Rope", -1, "layout %r, scaling %r" % (layout, scaling))
+        self.desc = _abi.RopeDesc(self.LAYOUTS[layout], rot_dim, theta, self.SCALINGS[scaling], factor, orig_ctx,
+                                  turns_fast, turns_slow, mscale)
 
 
 def prefill_ws_bytes(rows, K, T):

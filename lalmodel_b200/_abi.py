@@ -39,6 +39,22 @@ class Sampling(ctypes.Structure):
                 ("rep_penalty", c_float), ("no_repeat_ngram", c_int), ("n_masked_low_ids", c_int)]
 
 
+class KVBatchDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("n_seq", c_int), ("max_ctx", c_int), ("n_kv_head", c_int),
+                ("head_dim", c_int), ("k", P), ("v", P), ("row_pos", P), ("row_weight", P)]
+
+
+class RopeDesc(ctypes.Structure):
+    _fields_ = [("layout", c_int), ("rot_dim", c_int), ("theta", c_float), ("scaling", c_int),
+                ("factor", c_float), ("orig_ctx", c_float), ("turns_fast", c_float),
+                ("turns_slow", c_float), ("mscale", c_float)]
+
+
+class AttnBatchDesc(ctypes.Structure):
+    _fields_ = [("n_head", c_int), ("scale", c_float), ("prefix_len", c_int), ("prefix_k", P),
+                ("prefix_v", P), ("add_weights", c_int), ("decay", c_float)]
+
+
 # name -> (restype, argtypes); mirrors include/lalb.h one to one
 SIGNATURES = {
     "lalb_abi_version": (c_int, []),
@@ -65,6 +81,14 @@ SIGNATURES = {
     "lalb_decoder_set_position": (c_int, [P, c_int, P]),
     "lalb_decoder_position": (c_int, [P]),
     "lalb_attention_decode": (c_int, [P, P, c_int, c_int, c_int, c_int, c_int, c_float, P, P, P, P]),
+    "lalb_rope_append": (c_int, [P, ctypes.POINTER(RopeDesc), ctypes.POINTER(KVBatchDesc), c_int, P, c_int,
+                                 ctypes.c_longlong, c_int, P, P, P, P]),
+    "lalb_attention_batch_ws_bytes": (c_int, [ctypes.POINTER(KVBatchDesc), ctypes.POINTER(AttnBatchDesc),
+                                              ctypes.POINTER(c_size_t)]),
+    "lalb_attention_batch": (c_int, [P, ctypes.POINTER(KVBatchDesc), ctypes.POINTER(AttnBatchDesc), P,
+                                     ctypes.c_longlong, P, P, P, P]),
+    "lalb_kv_evict_ws_bytes": (c_int, [ctypes.POINTER(KVBatchDesc), c_int, ctypes.POINTER(c_size_t)]),
+    "lalb_kv_evict": (c_int, [P, ctypes.POINTER(KVBatchDesc), P, c_int, c_int, c_int, P, P]),
     "lalb_sample_ws_bytes": (c_int, [c_int, c_int, ctypes.POINTER(c_size_t)]),
     "lalb_blob_writer_open": (c_int, [ctypes.c_char_p, ctypes.POINTER(P)]),
     "lalb_blob_writer_add": (c_int, [P, ctypes.c_char_p, c_int, c_int, ctypes.POINTER(c_uint64), P]),
