@@ -2,117 +2,1073 @@
 // sequences that share a prefix (lalb_attention_batch), attention_forward
 // (runtime/lal_runtime.c:833-882) for many sequences at once.
 //
-// One CTA per (sequence, KV head), one warp per q head in turn: an online
-// softmax (running maximum and sum) over the prefix rows and the sequence's
-// own, fp32 throughout.
+//   out = sum_j 2^(x_j - M) v_j / sum_j 2^(x_j - M),  x_j = (scale log2 e) q . k_j
+//
+// over the prefix rows and the sequence's own.  Any set of rows j gives a
+// partial (m, l, O): a reference exponent m, l = sum_j 2^(x_j - m) and
+// O = sum_j 2^(x_j - m) v_j; partials over disjoint sets combine exactly.
+//
+// Units.  A prefix unit is a KV head and up to 128 query rows of ALL sequences
+// (row = sequence * group + head of the group) over the prefix, so its K and V
+// are read once for 128 rows instead of once per sequence.  An own unit is one
+// sequence's group of heads over its own rows.  Both are the same work: S =
+// Q K^T and O += P V with M = 128 rows on tcgen05, 64 cache rows (a tile) at a
+// time; an own unit fills only its group's lanes of the M = 128 instructions,
+// which costs tensor time that a memory-bound unit has to spare.
+//
+// Split.  All tiles of all units form one list, and CTA c of G (one per SM)
+// takes tiles [c W / G, (c + 1) W / G): equal shares whatever the lengths,
+// without the host knowing them.  A run of tiles of one unit in one CTA (a
+// segment) ends in one partial; attention_combine_kernel adds a row's partials
+// in list order, so results do not depend on scheduling.
+//
+// One CTA, warp-specialised (kSoftWarps softmax, 1 MMA, the loaders):
+//   loaders  K and V tiles into a ring, in the order K0 V0 K1 V1 ..; 16-bit
+//            caches by tiled TMA straight into the swizzled operand layout;
+//            F32 by eight warps that split each value into two fp16 parts;
+//   MMA      S(j+1) is issued before PV(j), so that the tensor cores work on
+//            the next scores while the softmax of this tile runs; Q is the A
+//            operand from TMEM, P overwrites its S in TMEM as the next A;
+//   softmax  two warpgroups on alternate tiles, each with its own O (128 rows
+//            = TMEM lanes = threads, so rows need no shuffles); O is rescaled
+//            only when a row's maximum has grown by more than 2^8.
+//
+// F32: x = hi + lo in fp16 (22 bits), three of the four products.  The eight
+// rows of a tile that a loader warp converts share a power of two that puts
+// their largest |x| in [2^14, 2^15); K's goes into the scores' factor, V's
+// exponent e into the weights' exponent: p' = 2^(x + e - m), v' = v 2^-e, so
+// that p' keeps its precision whatever the values' range, and l takes
+// p' 2^-e.  m is an integer: x + (e - m) then rounds once, at the size of the
+// exponent that matters.
+//
+// TMEM columns: S/P buffers 0..63 and 64..127, Q 128.., O up to 511.
+// Every wait is bounded.
+#include <cuda.h>
 #include <math.h>
 
 #include <algorithm>
 
 #include "lalb_batch.cuh"
+#include "lalb_tcgen05.cuh"
 
 using namespace lalb;
 
 namespace {
 
-constexpr int kAbWarps = 8;
+constexpr int kTile = 64;            // cache rows per tile
+constexpr int kM = 128;              // query rows per unit
+constexpr int kSide = 8;             // tiles whose F32 scales are kept (loaders run at most 5 ahead)
+constexpr float kShift = 6.0f;       // weights up to 2^6 at the reference maximum, 2^14 before a rescale
+constexpr float kGrow = 8.0f;        // growth of a row's maximum that is left in place
+constexpr int kColS = 0, kColQ = 128;
+constexpr int kStageBudget2 = 160 * 1024, kStageBudget1 = 192 * 1024;
+
+template <class T, int HD>
+struct Cfg {
+    static constexpr bool kF32 = sizeof(T) == 4;
+    // F32 at head_dim 256: Q's two parts take 256 TMEM columns, so a unit has
+    // half of the value columns (the scores are computed for both halves)
+    static constexpr int kDV = kF32 && HD == 256 ? 128 : HD;
+    static constexpr int kNDV = HD / kDV;
+    static constexpr int kQCols = kF32 ? HD : HD / 2;
+    static constexpr int kNS = kColQ + kQCols + 2 * kDV <= 512 ? 2 : 1;   // softmax streams
+    static constexpr int kColO = 512 - kNS * kDV;
+    static_assert(kColQ + kQCols <= kColO, "Q and O fit TMEM");
+    static constexpr int kSoftWarps = 4 * kNS;
+    // F32: 7, so that a block of two softmax warpgroups, the MMA warp and the
+    // loaders has 16 warps and 128 registers a thread
+    static constexpr int kLoadWarps = kF32 ? 7 : 1;
+    static constexpr int kFullCount = kF32 ? 8 : 1;    // arrivals that fill a stage: its groups of 8 rows
+    static constexpr int kThreads = 32 * (kSoftWarps + 1 + kLoadWarps);
+    static constexpr uint32_t kStage = kTile * HD * (kF32 ? 4 : 2);
+    static constexpr int kBudget = kNS == 2 ? kStageBudget2 : kStageBudget1;
+    static constexpr int kStages = kBudget / (int)kStage < 10 ? kBudget / (int)kStage : 10;
+    static_assert(kStages >= 3, "K(j), V(j) and K(j + 1) are held at once");
+    static_assert(kStages / 2 + 2 <= kSide, "a tile's scales outlive its stages");
+    static constexpr int kSubW = HD < 64 ? HD : 64;                   // columns of a swizzled subtile
+    static constexpr uint32_t kSub = kTile * kSubW * 2;               // its bytes
+    static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
+    static constexpr uint32_t kOffMl = kOffScratch + kSoftWarps * 4096;
+    static constexpr uint32_t kOffSide = kOffMl + 2 * kM * 8;
+    static constexpr uint32_t kOffBar = kOffSide + kSide * 16 * 4;
+    static constexpr uint32_t kSmem = 1024 + kOffBar + 512;
+    static_assert(kSmem <= 232448, "fits the 227 KB opt-in shared memory");
+    static_assert(kSmem > 116 * 1024 || kStages == 10, "one CTA per SM is what the ring is sized for");
+};
 
 struct AbArgs {
-    const void *q, *pk, *pv, *k, *v;
+    const void *q, *pk, *pv, *k, *v;   // pk .. v: F32 loaders only
     const int *lens;
+    int *cum;                    // [n_seq + 1] tiles of the sequences before b (one KV head's)
+    float *part_p, *part_o;      // partial O of prefix and own units
+    float2 *ml_p, *ml_o;         // their (m, l)
+    float *score;                // add_weights: x_j [n_seq][n_head][pitch]
     float *row_weight;
-    float2 *stat;                // [n_seq][n_head] (max, 1 / sum)
     void *out;
     unsigned int *status;
     long long q_stride;
-    int n_seq, n_head, n_kv, max_ctx, prefix, add_weights;
-    float scale, decay;
+    int n_seq, n_head, n_kv, group, hd, max_ctx, prefix, add_weights;
+    int m_p, m_o;                // 128-row tiles of a prefix and an own unit's KV head
+    int rows_p, rows_o;          // rows kept per partial
+    int ndv, grid, pitch;
+    float c, decay, sign;        // |scale| log2 e, sign of the scale
 };
 
-template <class T, int HD>
-__device__ __forceinline__ float ab_score(const float (&q)[HD / 32], const T *row, int lane) {
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) s = fmaf(q[i], to_f32<T>(row[lane + 32 * i]), s);
-    return warp_sum(s);
+__host__ __device__ inline int tiles_of(int rows) { return (rows + kTile - 1) / kTile; }
+
+__device__ __forceinline__ int own_len(const AbArgs &a, int b) {
+    const int n = __ldcg(a.lens + b);
+    return n < 0 || n > a.max_ctx ? 0 : n;
 }
 
-template <class T, int HD>
-__global__ void __launch_bounds__(32 * kAbWarps) attention_batch_kernel(const AbArgs a) {
-    __shared__ float2 stat[1024];
-    const int g = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int group = a.n_head / a.n_kv;
-    int n = a.lens[b];
-    if (n < 0 || n > a.max_ctx) {
-        if (threadIdx.x == 0) atomicOr(a.status, LALB_STATUS_BAD_POSITION);
-        n = 0;
+// The tile list: prefix tiles first, then per sequence its units.
+struct List {
+    long long tp, total;   // prefix tiles, all tiles
+    int lt;                // tiles of a prefix unit
+    int units_o;           // own units per sequence
+};
+
+__device__ __forceinline__ List make_list(const AbArgs &a, long long own_tiles) {
+    List l;
+    l.lt = tiles_of(a.prefix);
+    l.tp = (long long)a.n_kv * a.m_p * a.ndv * l.lt;
+    l.units_o = a.n_kv * a.m_o * a.ndv;
+    l.total = l.tp + own_tiles * l.units_o;
+    return l;
+}
+
+__device__ __forceinline__ long long cta_first(long long total, int grid, int c) {
+    return (total * c + grid - 1) / grid;
+}
+__device__ __forceinline__ int cta_of(long long total, int grid, long long t) { return (int)(t * grid / total); }
+
+struct Seg {
+    bool prefix;
+    int b;                 // own units: the sequence
+    int g, m, dv;
+    int j0, j1;            // tiles of the unit
+    int n;                 // rows of the unit's cache
+    int rows;              // query rows of the unit
+    long long slot;        // partial
+};
+
+// Walks one CTA's segments.  Every role walks on its own.
+struct Walk {
+    long long t, end;
+    int b;
+    long long c0;          // list position of sequence b's first own tile, less tp
+    int n, nt;             // length and tiles of sequence b
+
+    __device__ __forceinline__ bool next(const AbArgs &a, const List &l, Seg &s) {
+        if (t >= end) return false;
+        int u, units;
+        if (t < l.tp) {
+            u = (int)(t / l.lt);
+            s.prefix = true;
+            s.j0 = (int)(t % l.lt);
+            s.j1 = (int)min((long long)l.lt, s.j0 + (min(end, l.tp) - t));
+            s.n = a.prefix;
+            s.slot = (long long)blockIdx.x + u;
+            units = a.m_p;
+            s.b = 0;
+        } else {
+            const long long o = t - l.tp;
+            while (o >= c0 + (long long)nt * l.units_o) {
+                c0 += (long long)nt * l.units_o;
+                ++b;
+                n = own_len(a, b);
+                nt = tiles_of(n);
+            }
+            u = (int)((o - c0) / nt);
+            s.prefix = false;
+            s.j0 = (int)((o - c0) % nt);
+            s.j1 = (int)min((long long)nt, s.j0 + (end - t));
+            s.n = n;
+            s.slot = (long long)blockIdx.x + (long long)b * l.units_o + u;
+            units = a.m_o;
+            s.b = b;
+        }
+        s.dv = u % a.ndv;
+        s.m = u / a.ndv % units;
+        s.g = u / a.ndv / units;
+        s.rows = min(kM, (s.prefix ? a.n_seq * a.group : a.group) - s.m * kM);
+        t += s.j1 - s.j0;
+        return true;
     }
-    const size_t kvr = (size_t)a.n_kv * HD;
-    const T *pk = static_cast<const T *>(a.pk), *pv = static_cast<const T *>(a.pv);
-    const T *k = static_cast<const T *>(a.k) + (size_t)b * a.max_ctx * kvr;
-    const T *v = static_cast<const T *>(a.v) + (size_t)b * a.max_ctx * kvr;
-    for (int hh = warp; hh < group; hh += kAbWarps) {
-        const int h = g * group + hh;
-        const T *qp = static_cast<const T *>(a.q) + (size_t)b * a.q_stride + (size_t)h * HD;
-        float q[HD / 32], acc[HD / 32];
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-            q[i] = to_f32<T>(qp[lane + 32 * i]) * a.scale;
-            acc[i] = 0.0f;
-        }
-        float m = -INFINITY, l = 0.0f;
-        for (int j = 0; j < a.prefix + n; ++j) {
-            const size_t off = (size_t)(j < a.prefix ? j : j - a.prefix) * kvr + (size_t)g * HD;
-            const float s = ab_score<T, HD>(q, (j < a.prefix ? pk : k) + off, lane);
-            const T *vr = (j < a.prefix ? pv : v) + off;
-            const float mn = fmaxf(m, s), c = expf(m - mn), p = expf(s - mn);
-            m = mn;
-            l = fmaf(l, c, p);
-#pragma unroll
-            for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(acc[i], c, p * to_f32<T>(vr[lane + 32 * i]));
-        }
-        T *o = static_cast<T *>(a.out) + (size_t)b * a.n_head * HD + (size_t)h * HD;
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) o[lane + 32 * i] = from_f32<T>(acc[i] * inv);
-        if (lane == 0 && hh < 1024) stat[hh] = make_float2(m, inv);
-    }
-    if (!a.add_weights) return;
-    __syncthreads();
-    for (int j = warp; j < n; j += kAbWarps) {
-        float w = 0.0f;
-        for (int hh = 0; hh < group; ++hh) {
-            const T *qp = static_cast<const T *>(a.q) + (size_t)b * a.q_stride + (size_t)(g * group + hh) * HD;
-            float q[HD / 32];
-#pragma unroll
-            for (int i = 0; i < HD / 32; ++i) q[i] = to_f32<T>(qp[lane + 32 * i]) * a.scale;
-            w += expf(ab_score<T, HD>(q, k + (size_t)j * kvr + (size_t)g * HD, lane) - stat[hh].x) * stat[hh].y;
-        }
-        if (lane == 0) {
-            float *r = a.row_weight + ((size_t)b * a.n_kv + g) * a.max_ctx + j;
-            *r = a.decay == 0.0f ? w : fmaf(a.decay, *r, w);
-        }
-    }
+};
+
+// ---- small PTX helpers -----------------------------------------------------------
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, float *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
 }
 
 template <class T>
-const void *ab_kernel(int hd) {
-    switch (hd) {
-        case 32: return (const void *)attention_batch_kernel<T, 32>;
-        case 64: return (const void *)attention_batch_kernel<T, 64>;
-        case 128: return (const void *)attention_batch_kernel<T, 128>;
-        default: return (const void *)attention_batch_kernel<T, 256>;
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// x0, x1 as two 16-bit parts each: returns the pair of high parts, lo the rest.
+template <class H>
+__device__ __forceinline__ uint32_t split2(float x0, float x1, uint32_t &lo) {
+    const uint32_t h = pack2<H>(x0, x1);
+    float h0, h1;
+    if constexpr (std::is_same<H, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+        h0 = f.x, h1 = f.y;
+    } else {
+        h0 = __uint_as_float(h << 16), h1 = __uint_as_float(h & 0xffff0000u);
+    }
+    lo = pack2<H>(x0 - h0, x1 - h1);
+    return h;
+}
+
+// Exponent e, 2^e the power of two that v 2^-e puts |v| <= amax below 2^15
+// (and amax at or above 2^14), held in a range where 2^e and 2^-e stay normal.
+__device__ __forceinline__ int part_exponent(float amax) {
+    const int e = (int)(__float_as_uint(amax) >> 23) - 127 - 14;
+    return min(max(e, -74), 113);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// K-major tile (rows = tile rows, swizzled rows of kSubW 16-bit columns).
+template <int SUBW>
+__device__ __forceinline__ uint64_t kmajor_desc(uint32_t saddr) {
+    constexpr uint64_t sbo = SUBW * 2 * 8, type = SUBW == 64 ? 2 : 4;
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((sbo >> 4) << 32) | ((uint64_t)1 << 46) |
+           (type << 61);
+}
+// The same bytes read along the rows: columns are N, tile rows are K.  The
+// next 64 columns are one subtile on, the next 8 rows one swizzle atom.
+template <int SUBW>
+__device__ __forceinline__ uint64_t mnmajor_desc(uint32_t saddr) {
+    constexpr uint64_t sbo = SUBW * 2 * 8, type = SUBW == 64 ? 2 : 4, lbo = kTile * SUBW * 2;
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((lbo >> 4) << 16) | ((sbo >> 4) << 32) | ((uint64_t)1 << 46) |
+           (type << 61);
+}
+
+template <class T>
+constexpr uint32_t mma_idesc(int n, bool b_mn) {
+    const uint32_t t = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;   // bf16 : fp16
+    return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(kM >> 4) << 24);
+}
+
+// ---- F32 loaders: eight rows of a tile by one warp -------------------------------------
+// Rows r0 .. r0 + 7 of the tile (cache rows row0 + r0 ..; rows at or past n
+// are zeros), COLS columns from src: registers first, then split and stored.
+template <int COLS>
+struct RowLoad {
+    static constexpr int kLanes = COLS / 4 < 32 ? COLS / 4 : 32;   // lanes of one row
+    static constexpr int kPer = 32 / kLanes;                       // rows per load
+    static constexpr int kVec = COLS / (4 * kLanes);               // loads of one row
+    static constexpr int kN = 8 / kPer * kVec;
+    float4 x[kN];
+
+    __device__ __forceinline__ void load(const float *src, size_t pitch, int left, int lane) {
+        const int rr = lane / kLanes, cc = (lane % kLanes) * 4;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int r = i / kVec * kPer + rr, c = cc + (i % kVec) * 4 * kLanes;
+            x[i] = r < left ? __ldg(reinterpret_cast<const float4 *>(src + (size_t)r * pitch + c))
+                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
+    // The rows' common exponent.
+    __device__ __forceinline__ int exponent() const {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            m = fmaxf(m, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+        return part_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+    }
+    __device__ __forceinline__ void store(uint8_t *stage, int r0, float scale, int lane) const {
+        constexpr int W = COLS < 64 ? COLS : 64;
+        constexpr uint32_t kLo = kTile * COLS * 2;
+        const int rr = lane / kLanes, cc = (lane % kLanes) * 4;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int r = r0 + i / kVec * kPer + rr, c = cc + (i % kVec) * 4 * kLanes;
+            uint2 hi, lo;
+            hi.x = split2<__half>(x[i].x * scale, x[i].y * scale, lo.x);
+            hi.y = split2<__half>(x[i].z * scale, x[i].w * scale, lo.y);
+            const int unit = (c % W) >> 3;
+            const int sw = W == 64 ? unit ^ (r & 7) : unit ^ ((r >> 1) & 3);
+            const uint32_t off = (uint32_t)(c / W) * (kTile * W * 2) + r * (W * 2) + sw * 16 + (c & 4) * 2;
+            *reinterpret_cast<uint2 *>(stage + off) = hi;
+            *reinterpret_cast<uint2 *>(stage + off + kLo) = lo;
+        }
+    }
+};
+
+template <class T, int HD>
+__global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
+    attention_tiles_kernel(const __grid_constant__ CUtensorMap mPK, const __grid_constant__ CUtensorMap mPV,
+                           const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
+                           const __grid_constant__ AbArgs a) {
+    using C = Cfg<T, HD>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    float2 *ml = reinterpret_cast<float2 *>(smem + C::kOffMl);        // [stream][row]
+    float *side = reinterpret_cast<float *>(smem + C::kOffSide);      // [tile % kSide][K 8, V 8]
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
+    uint64_t *empty = full + C::kStages;
+    uint64_t *sfull = empty + C::kStages;      // S(j) complete (and every product before it)
+    uint64_t *pready = sfull + 2;              // P(j) written
+    uint64_t *ofull = pready + 2;              // a stream's latest PV complete
+    uint64_t *qready = ofull + 2;              // Q of the segment written, O of the last one read
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(qready + 1);
+    int *start_b = reinterpret_cast<int *>(tmem_slot + 1);
+    long long *start = reinterpret_cast<long long *>(start_b + 1);    // own tiles of all, of those before start_b
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], C::kFullCount);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&sfull[s], 1);
+            mbar_init(&pready[s], 4);
+            mbar_init(&ofull[s], 1);
+        }
+        mbar_init(qready, C::kSoftWarps);
+        fence_barrier_init();
+    }
+    if (warp == C::kSoftWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_before();
+    }
+    pdl_wait();
+    // ---- the list: its length, and where this CTA's own tiles begin ---------------------
+    if (warp == 0) {
+        long long sum = 0;
+        for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+            const int b = b0 + lane;
+            int nt = 0;
+            if (b < a.n_seq) {
+                const int n = __ldcg(a.lens + b);
+                if (n < 0 || n > a.max_ctx) {
+                    if (blockIdx.x == 0) atomicOr(a.status, LALB_STATUS_BAD_POSITION);
+                } else {
+                    nt = tiles_of(n);
+                }
+            }
+            int incl = nt;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            if (blockIdx.x == 0 && b < a.n_seq) a.cum[b] = (int)sum + incl - nt;
+            sum += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (blockIdx.x == 0 && lane == 0) a.cum[a.n_seq] = (int)sum;
+        const List l = make_list(a, sum);
+        const long long first = cta_first(l.total, a.grid, blockIdx.x) - l.tp;   // among the own tiles
+        // the sequence of that tile (of the first one, if the CTA begins in the prefix)
+        int sb = 0;
+        long long before = 0;
+        if (first > 0 && first < sum * l.units_o) {
+            const long long want = first / l.units_o;     // cum[sb] <= want < cum[sb + 1]
+            long long run = 0;
+            for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+                const int b = b0 + lane;
+                const int nt = b < a.n_seq ? tiles_of(own_len(a, b)) : 0;
+                int incl = nt;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += x;
+                }
+                const uint32_t past = __ballot_sync(0xffffffffu, run + incl > want);
+                if (past) {
+                    const int i = __ffs(past) - 1;
+                    sb = b0 + i;
+                    before = run + __shfl_sync(0xffffffffu, incl - nt, i);
+                    break;
+                }
+                run += __shfl_sync(0xffffffffu, incl, 31);
+            }
+        }
+        if (lane == 0) {
+            *start_b = sb;
+            start[0] = sum;
+            start[1] = before;
+        }
+    }
+    __syncthreads();
+    pdl_launch_dependents();   // after the allocation: a dependent that allocates TMEM too must not come first
+    tc_after();
+    const uint32_t tmem = *tmem_slot;
+    // with the whole of TMEM allocated its base is column 0; anything else
+    // raises a status bit and skips the work
+    const bool tmem_ok = tmem == 0;
+    if (!tmem_ok && threadIdx.x == 0) atomicOr(a.status, LALB_STATUS_WAIT_TIMEOUT);
+    const List list = make_list(a, start[0]);
+    Walk walk;
+    walk.t = list.total ? cta_first(list.total, a.grid, blockIdx.x) : 0;
+    walk.end = list.total && tmem_ok ? cta_first(list.total, a.grid, blockIdx.x + 1) : 0;
+    walk.b = *start_b;
+    walk.c0 = start[1] * list.units_o;
+    walk.n = own_len(a, walk.b);
+    walk.nt = tiles_of(walk.n);
+    Seg s;
+
+    if (warp > C::kSoftWarps) {
+        // ================================ loaders ===============================================
+        if constexpr (C::kF32) {
+            // a stage is 8 groups of 8 rows; the groups go round the loader warps
+            const int w = warp - C::kSoftWarps - 1;
+            const size_t pitch = (size_t)a.n_kv * HD;
+            uint32_t st = 0, tile = 0;     // stages and tiles so far
+            uint32_t turn = w;             // the first group of stage st that is this warp's
+            bool ok = true;
+            auto group = [&](auto &x, const float *base, int j, int n, int g) {
+                const size_t row = (size_t)j * kTile + 8 * g;
+                x.load(base + row * pitch, pitch, n - (int)row, lane);
+            };
+            auto finish = [&](auto &x, int g, bool is_v) {
+                const int e = x.exponent();
+                const uint32_t slot = st % C::kStages, use = st / C::kStages;
+                if (use > 0) ok = ok && warp_wait_fast(&empty[slot], (use - 1) & 1u, a.status);
+                x.store(smem + slot * C::kStage, 8 * g, pow2(-e), lane);
+                // K: the factor that undoes the scaling; V: the exponent
+                if (lane == 0) side[(tile % kSide) * 16 + (is_v ? 8 : 0) + g] = is_v ? (float)e : pow2(e);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[slot]);
+            };
+            while (walk.next(a, list, s)) {
+                const size_t seq = s.prefix ? 0 : (size_t)s.b * a.max_ctx * pitch;
+                const float *kb = static_cast<const float *>(s.prefix ? a.pk : a.k) + seq + (size_t)s.g * HD;
+                const float *vb =
+                    static_cast<const float *>(s.prefix ? a.pv : a.v) + seq + (size_t)s.g * HD + s.dv * C::kDV;
+                for (int j = s.j0; j < s.j1 && ok; ++j, ++tile) {
+                    for (int g = turn; g < 8; g += C::kLoadWarps) {
+                        RowLoad<HD> x;
+                        group(x, kb, j, s.n, g);
+                        finish(x, g, false);
+                    }
+                    ++st;
+                    turn = (turn + 6) % 7;          // 8 groups on: -8 = 6 mod 7
+                    for (int g = turn; g < 8; g += C::kLoadWarps) {
+                        RowLoad<C::kDV> x;
+                        group(x, vb, j, s.n, g);
+                        finish(x, g, true);
+                    }
+                    ++st;
+                    turn = (turn + 6) % 7;
+                }
+            }
+        } else if (lane == 0) {
+            uint32_t st = 0;
+            bool ok = true;
+            while (walk.next(a, list, s)) {
+                const CUtensorMap *mk = s.prefix ? &mPK : &mK, *mv = s.prefix ? &mPV : &mV;
+                const int row0 = s.prefix ? 0 : s.b * a.max_ctx;
+                for (int j = s.j0; j < s.j1 && ok; ++j)
+                    for (int kv = 0; kv < 2 && ok; ++kv, ++st) {
+                        const uint32_t slot = st % C::kStages, use = st / C::kStages;
+                        if (use > 0 && !mbar_wait_bounded(&empty[slot], (use - 1) & 1u, a.status)) {
+                            ok = false;
+                            break;
+                        }
+                        mbar_arrive_expect_tx(&full[slot], C::kStage);
+#pragma unroll
+                        for (int c = 0; c < HD / C::kSubW; ++c)
+                            tma2d(smem + slot * C::kStage + c * C::kSub, kv ? mv : mk, s.g * HD + c * C::kSubW,
+                                  row0 + j * kTile, &full[slot]);
+                    }
+            }
+            // nothing may still be on its way into this CTA's shared memory when it ends
+            for (uint32_t i = st > (uint32_t)C::kStages ? st - C::kStages : 0; i < st; ++i)
+                mbar_wait_bounded(&full[i % C::kStages], (i / C::kStages) & 1u, a.status);
+        }
+    } else if (warp == C::kSoftWarps) {
+        // ================================ MMA ====================================================
+        constexpr uint32_t kIdS = mma_idesc<typename std::conditional<C::kF32, __half, T>::type>(kTile, false);
+        constexpr uint32_t kIdO = mma_idesc<typename std::conditional<C::kF32, __half, T>::type>(C::kDV, true);
+        constexpr uint32_t kLoK = kTile * HD * 2, kLoV = kTile * C::kDV * 2;
+        const uint32_t ring = smem_u32(smem);
+        uint32_t st = 0, tile = 0, segs = 0;
+        uint32_t vslot = 0;
+        bool ok = true;
+        auto issue_pv = [&](uint32_t t, uint32_t sv, uint32_t sv_use, bool first) -> bool {
+            const uint32_t buf = t & 1u;
+            if (!warp_wait_fast(&pready[buf], (t >> 1) & 1u, a.status) ||
+                !warp_wait_fast(&full[sv], sv_use & 1u, a.status))
+                return false;
+            tc_after();
+            const uint32_t stream = C::kNS == 2 ? buf : 0;
+            const uint32_t d = C::kColO + stream * C::kDV, p = kColS + buf * kTile, v = ring + sv * C::kStage;
+            // weights: high parts at 32 h + 0..15 of the buffer, the rest 16 columns on
+            auto hi = [&](int kk) { return p + 32 * (kk >> 1) + 8 * (kk & 1); };
+            auto v_off = [&](int kk) { return v + kk * 16 * C::kSubW * 2; };
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk) {
+                if constexpr (C::kF32)
+                    mma_f16_ta(d, hi(kk), mnmajor_desc<C::kSubW>(v_off(kk) + kLoV), kIdO, first && kk == 0 ? 0u : 1u);
+                mma_f16_ta(d, hi(kk) + 16, mnmajor_desc<C::kSubW>(v_off(kk)), kIdO,
+                           first && kk == 0 && !C::kF32 ? 0u : 1u);
+            }
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk)
+                mma_f16_ta(d, hi(kk), mnmajor_desc<C::kSubW>(v_off(kk)), kIdO, 1u);
+            commit_elect(&empty[sv]);
+            commit_elect(&ofull[stream]);
+            return true;
+        };
+        while (ok && walk.next(a, list, s)) {
+            if (!(ok = warp_wait_fast(qready, segs & 1u, a.status))) break;
+            tc_after();
+            ++segs;
+            const int n = s.j1 - s.j0;
+            for (int i = 0; i <= n; ++i) {
+                if (i < n) {
+                    const uint32_t t = tile + i, buf = t & 1u;
+                    const uint32_t sk = st % C::kStages, use = st / C::kStages;
+                    if (!(ok = warp_wait_fast(&full[sk], use & 1u, a.status))) break;
+                    tc_after();
+                    const uint32_t d = kColS + buf * kTile, k = ring + sk * C::kStage;
+                    auto k_off = [&](int kk) {
+                        return k + (kk / (C::kSubW / 16)) * C::kSub + (kk % (C::kSubW / 16)) * 32;
+                    };
+                    // The tensor cores cut each sum off towards zero at its own size: the
+                    // small products go first, while the sum is small (at head_dim 256,
+                    // in the middle of the large ones: 3x the output error).
+                    if constexpr (C::kF32) {
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            mma_f16_ta(d, kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS, kk ? 1u : 0u);
+                            mma_f16_ta(d, kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, 1u);
+                        }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk)
+                        mma_f16_ta(d, kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, kk || C::kF32 ? 1u : 0u);
+                    commit_elect(&empty[sk]);
+                    commit_elect(&sfull[buf]);
+                }
+                if (i > 0) {
+                    // tile i - 1's values: the stage before K(i) (the last one: before the end)
+                    const uint32_t v = vslot;
+                    const bool first = i - 1 < C::kNS;
+                    if (!(ok = issue_pv(tile + i - 1, v % C::kStages, v / C::kStages, first))) break;
+                }
+                vslot = st + 1;
+                if (i < n) st += 2;
+            }
+            tile += n;
+        }
+    } else {
+        // ================================ softmax ==================================================
+        const int wg = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        uint8_t *scratch = smem + C::kOffScratch + warp * 4096;
+        uint32_t tile = 0, st = 0;              // before the segment
+        uint32_t pv[2] = {0, 0};                // products of each stream so far
+        bool ok = true;
+        auto soft_bar = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kSoftWarps) : "memory"); };
+        while (walk.next(a, list, s)) {
+            const int n = s.j1 - s.j0;
+            const bool active = quarter * 32 < s.rows;    // a row of this warp belongs to the unit
+            const bool mine = row < s.rows;
+            // ---- Q: this warp's rows, the columns of its warpgroup, into TMEM ------------------
+            float cq = a.c;                               // score factor of this thread's row
+            if (active) {
+                const T *qb = static_cast<const T *>(a.q) + (size_t)s.g * a.group * HD;
+                auto q_row = [&](int r) -> const T * {    // query row r of the unit
+                    const int rr = s.m * kM + r;
+                    const int b = s.prefix ? rr / a.group : s.b, h = s.prefix ? rr % a.group : rr;
+                    return qb + (size_t)b * a.q_stride + (size_t)h * HD;
+                };
+                constexpr int kLpr = 2 * sizeof(T);       // lanes per row of a 32-column chunk
+                constexpr int kRpi = 32 / kLpr;
+                const int lr = lane / kLpr, lu = lane % kLpr;
+                const int live = min(32, s.rows - quarter * 32);
+                float qs = a.sign;
+                if constexpr (C::kF32) {
+                    // the row's largest value, by the lanes that read it side by side
+                    float mine_max = 0.0f;
+                    for (int r = 0; r < live; r += kRpi) {
+                        float m = 0.0f;
+                        if (r + lr < live) {
+                            const float *p = reinterpret_cast<const float *>(q_row(quarter * 32 + r + lr)) + lu * 4;
+#pragma unroll
+                            for (int c = 0; c < HD / 32; ++c) {
+                                const float4 v = __ldg(reinterpret_cast<const float4 *>(p + 32 * c));
+                                m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                            }
+                        }
+#pragma unroll
+                        for (int o = 1; o < kLpr; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        const float x = __shfl_sync(0xffffffffu, m, ((lane - r) & (kRpi - 1)) * kLpr);
+                        if (lane >= r && lane < r + kRpi) mine_max = x;
+                    }
+                    const int e = part_exponent(mine_max);
+                    qs = a.sign * pow2(-e);
+                    cq = a.c * pow2(e);
+                }
+                for (int c = wg; c < HD / 32; c += C::kNS) {
+                    for (int r = 0; r < live; r += kRpi)
+                        if (r + lr < live) {
+                            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(q_row(quarter * 32 + r + lr) + 32 * c) + lu);
+                            *reinterpret_cast<uint4 *>(scratch + (r + lr) * 128 + ((lu ^ ((r + lr) & 7)) << 4)) = v;
+                        }
+                    __syncwarp();
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int u = 0; u < kLpr; ++u) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4));
+                        if constexpr (C::kF32) {
+                            hi[2 * u] = split2<__half>(__uint_as_float(v.x) * qs, __uint_as_float(v.y) * qs, lo[2 * u]);
+                            hi[2 * u + 1] = split2<__half>(__uint_as_float(v.z) * qs, __uint_as_float(v.w) * qs, lo[2 * u + 1]);
+                        } else {
+                            // a negative scale turns the queries' signs
+                            const uint32_t f = qs < 0.0f ? 0x80008000u : 0u;
+                            hi[4 * u] = v.x ^ f, hi[4 * u + 1] = v.y ^ f, hi[4 * u + 2] = v.z ^ f, hi[4 * u + 3] = v.w ^ f;
+                        }
+                    }
+                    tmem_st16(lanes + kColQ + 16 * c, hi);
+                    if constexpr (C::kF32) tmem_st16(lanes + kColQ + HD / 2 + 16 * c, lo);
+                    __syncwarp();
+                }
+                tmem_wait_st();
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(qready);
+
+            // ---- this warpgroup's tiles ----------------------------------------------------------
+            float mref = 0.0f, l = 0.0f;
+            bool any = false, had = false;
+            float *score = nullptr;
+            if (a.add_weights && !s.prefix && s.dv == 0 && mine)
+                score = a.score + ((size_t)s.b * a.n_head + (size_t)s.g * a.group + s.m * kM + row) * a.pitch;
+            for (int i = 0; i < n; ++i) {
+                const uint32_t t = tile + i, buf = t & 1u;
+                const uint32_t stream = C::kNS == 2 ? buf : 0;
+                const uint32_t sk = st + 2 * i, sv = sk + 1;
+                const bool my_tile = C::kNS == 1 || (int)buf == wg;
+                if (my_tile) {
+                    // This stream's last product complete.  With two streams S(t)
+                    // complete already means it (it was issued first); with one
+                    // stream every product is waited for, so that the barrier
+                    // is never two phases ahead of a wait.
+                    bool waited = C::kNS == 2 || pv[stream] == 0;
+                    auto wait_pv = [&]() {
+                        if (!waited) ok = ok && warp_wait_fast(&ofull[stream], (pv[stream] - 1) & 1u, a.status);
+                        waited = true;
+                        tc_after();
+                    };
+                    had = true;
+                    const int valid = s.n - (s.j0 + i) * kTile;     // of the tile's 64 rows
+                    ok = ok && warp_wait_fast(&sfull[buf], (t >> 1) & 1u, a.status);
+                    tc_after();
+                    if constexpr (!C::kF32) {
+                        // stale rows behind a sequence's end may hold anything, NaN too,
+                        // and 0 x NaN is NaN: the values' tile gets zeros there
+                        if (!s.prefix && valid < kTile) {
+                            ok = ok && warp_wait_fast(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
+                            uint8_t *v = smem + (sv % C::kStages) * C::kStage;
+                            constexpr int kU = C::kSubW * 2 / 16;
+                            const int units = (kTile - valid) * kU * (HD / C::kSubW);
+                            for (int u = quarter * 32 + lane; u < units; u += 128) {
+                                const int c = u / ((kTile - valid) * kU), r = u % ((kTile - valid) * kU);
+                                *reinterpret_cast<uint4 *>(v + c * C::kSub + valid * C::kSubW * 2 + r * 16) =
+                                    make_uint4(0, 0, 0, 0);
+                            }
+                            fence_async();
+                        }
+                    } else {
+                        ok = ok && warp_wait_fast(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
+                    }
+                    if (active && ok) {
+                        const uint32_t sc = lanes + kColS + buf * kTile;
+                        float x[kTile];
+                        tmem_ld32_nowait(sc, x);
+                        tmem_ld32_nowait(sc + 32, x + 32);
+                        tmem_wait_ld();
+                        if (valid < kTile) {
+#pragma unroll
+                            for (int j = 0; j < kTile; ++j)
+                                if (j >= valid) x[j] = -INFINITY;
+                        }
+                        float top = -INFINITY;
+                        const float *sd = side + (t % kSide) * 16;
+                        // never 0: -inf (a row past the end) times it has to stay -inf
+                        auto factor = [&](int g) { return fmaxf(sd[g] * cq, 1e-37f); };
+                        if constexpr (C::kF32) {
+#pragma unroll
+                            for (int g = 0; g < 8; ++g) {
+                                const float f = factor(g), e = sd[8 + g];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) top = fmaxf(top, fmaf(x[8 * g + j], f, e));
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < kTile; ++j) top = fmaxf(top, x[j]);
+                            top *= cq;
+                        }
+                        if (score) {
+                            float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile);
+#pragma unroll
+                            for (int j = 0; j < kTile; j += 4) {
+                                const float f = C::kF32 ? factor(j >> 3) : cq;
+                                o[j >> 2] = make_float4(x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f);
+                            }
+                        }
+                        // ---- the reference exponent ----------------------------------------------------
+                        const float want = top == -INFINITY ? (any ? mref : 0.0f) : rintf(top) - kShift;
+                        if (!any) {
+                            mref = want;
+                        } else if (__any_sync(0xffffffffu, want > mref + kGrow)) {
+                            wait_pv();
+                            const float to = want > mref + kGrow ? want : mref;
+                            const float f = ex2(mref - to);
+                            mref = to;
+                            l *= f;
+                            const uint32_t oc = lanes + C::kColO + stream * C::kDV;
+#pragma unroll
+                            for (int c = 0; c < C::kDV; c += 32) {
+                                float o[32];
+                                tmem_ld32_nowait(oc + c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] *= f;
+                                tmem_st32(oc + c, *reinterpret_cast<const uint32_t(*)[32]>(o));
+                            }
+                        }
+                        // ---- weights -------------------------------------------------------------------
+                        if constexpr (C::kF32) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t w[32];
+#pragma unroll
+                                for (int g = 4 * h; g < 4 * h + 4; ++g) {
+                                    const float f = factor(g), e = sd[8 + g] - mref;
+                                    float sum = 0.0f;
+#pragma unroll
+                                    for (int j = 0; j < 8; j += 2) {
+                                        const float p0 = ex2(fmaf(x[8 * g + j], f, e));
+                                        const float p1 = ex2(fmaf(x[8 * g + j + 1], f, e));
+                                        sum += p0 + p1;
+                                        const int o = 4 * (g - 4 * h) + (j >> 1);
+                                        w[o] = split2<__half>(p0, p1, w[16 + o]);
+                                    }
+                                    l = fmaf(sum, pow2(-(int)sd[8 + g]), l);
+                                }
+                                tmem_st32(sc + 32 * h, w);
+                            }
+                        } else {
+                            float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t w[32];
+#pragma unroll
+                                for (int j = 0; j < 32; j += 2) {
+                                    const float p0 = ex2(fmaf(x[32 * h + j], cq, -mref));
+                                    const float p1 = ex2(fmaf(x[32 * h + j + 1], cq, -mref));
+                                    l0 += p0;
+                                    l1 += p1;
+                                    w[j >> 1] = split2<T>(p0, p1, w[16 + (j >> 1)]);
+                                }
+                                tmem_st32(sc + 32 * h, w);
+                            }
+                            l += l0 + l1;
+                        }
+                        tmem_wait_st();
+                        any = true;
+                    }
+                    wait_pv();
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&pready[buf]);
+                }
+                ++pv[stream];
+            }
+
+            // ---- the segment's partial: both streams' sums --------------------------------------------
+            // each warpgroup waits for its own stream's last product
+            {
+                const uint32_t k = C::kNS == 2 ? wg : 0;
+                if (had) ok = ok && warp_wait_fast(&ofull[k], (pv[k] - 1) & 1u, a.status);
+            }
+            tc_before();
+            ml[wg * kM + row] = make_float2(mref, l);
+            soft_bar();
+            tc_after();
+            float2 r0 = ml[row], r1 = C::kNS == 2 ? ml[kM + row] : make_float2(0.0f, 0.0f);
+            // a stream without a tile in this segment has nothing (the other has)
+            const bool has0 = C::kNS == 1 || n > 1 || (tile & 1u) == 0, has1 = C::kNS == 2 && (n > 1 || (tile & 1u) == 1);
+            const float m = has0 && has1 ? fmaxf(r0.x, r1.x) : has0 ? r0.x : r1.x;
+            const float f0 = has0 ? ex2(r0.x - m) : 0.0f, f1 = has1 ? ex2(r1.x - m) : 0.0f;
+            if (active && ok) {
+                const int rows = s.prefix ? a.rows_p : a.rows_o;
+                const size_t first = (size_t)s.slot * rows + quarter * 32;
+                float *po = (s.prefix ? a.part_p : a.part_o) + first * C::kDV;
+                float2 *pm = (s.prefix ? a.ml_p : a.ml_o) + first;
+                const int live = min(32, s.rows - quarter * 32);
+                if (wg == 0 && mine)
+                    pm[lane] = make_float2(m, (has0 ? r0.y * f0 : 0.0f) + (has1 ? r1.y * f1 : 0.0f));
+                constexpr int kHalf = C::kDV / C::kNS, kP = kHalf < 32 ? kHalf : 32;
+                constexpr int kLpr = kP / 4, kRpi = 32 / kLpr;
+                const int lr = lane / kLpr, lu = lane % kLpr;
+#pragma unroll 1
+                for (int c = wg * kHalf; c < (wg + 1) * kHalf; c += kP) {
+                    float o[kP];
+#pragma unroll
+                    for (int k = 0; k < kP; ++k) o[k] = 0.0f;
+                    if (has0) {
+                        float v[16];
+#pragma unroll
+                        for (int k = 0; k < kP; k += 16) {
+                            tmem_ld16(lanes + C::kColO + c + k, v);
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) o[k + q] = v[q] * f0;
+                        }
+                    }
+                    if (has1) {
+                        float v[16];
+#pragma unroll
+                        for (int k = 0; k < kP; k += 16) {
+                            tmem_ld16(lanes + C::kColO + C::kDV + c + k, v);
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) o[k + q] = fmaf(v[q], f1, o[k + q]);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < kLpr; ++u)
+                        *reinterpret_cast<float4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4)) =
+                            make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                    __syncwarp();
+                    for (int r = 0; r < live; r += kRpi)
+                        if (r + lr < live)
+                            *reinterpret_cast<float4 *>(po + (size_t)(r + lr) * C::kDV + c + 4 * lu) =
+                                *reinterpret_cast<const float4 *>(scratch + (r + lr) * 128 + ((lu ^ ((r + lr) & 7)) << 4));
+                    __syncwarp();
+                }
+            }
+            tc_before();
+            soft_bar();      // ml is free, and no warp writes Q while another reads O
+            tile += n;
+            st += 2 * n;
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == C::kSoftWarps) {
+        __syncwarp();
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
 }
+
+// ---- the rows' partials together, and the rows' weights -----------------------------------------
+constexpr int kCombWarps = 8;
+constexpr int kMaxGroup = 1024;
+
+// Runs over the partials of one unit: tiles [t, t + nt) of the list.
+template <class F>
+__device__ __forceinline__ void each_partial(const AbArgs &a, long long total, long long t, int nt, long long unit,
+                                             F f) {
+    const int c0 = cta_of(total, a.grid, t), c1 = cta_of(total, a.grid, t + nt - 1);
+    for (int c = c0; c <= c1; ++c) {
+        // a CTA between them may have no tile at all
+        if (cta_first(total, a.grid, c) < cta_first(total, a.grid, c + 1)) f(c + unit);
+    }
+}
+
+// CTA (KV head g, sequence b, z): warps take the group's heads; z = 0 writes
+// the outputs, and all z share the rows whose weights are kept.
+template <class T, int HD>
+__global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(const __grid_constant__ AbArgs a) {
+    using C = Cfg<T, HD>;
+    constexpr int kVec = C::kDV / 32;     // value columns per lane
+    __shared__ float2 stat[kMaxGroup];    // (M, 1 / L) of each head of the group
+    const int g = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int cum = __ldcg(a.cum + b), nt = __ldcg(a.cum + b + 1) - cum;
+    const List l = make_list(a, __ldcg(a.cum + a.n_seq));
+    const int n_out = blockIdx.z == 0 ? C::kNDV : 1;    // the weights need one half's sums only
+    for (int i = warp; i < a.group * n_out; i += kCombWarps) {
+        const int hh = i / n_out, dv = i % n_out;
+        const int rp = b * a.group + hh;
+        const long long up = ((long long)g * a.m_p + rp / kM) * a.ndv + dv;
+        const long long uo = ((long long)g * a.m_o + hh / kM) * a.ndv + dv;
+        const long long tp = up * l.lt, to = l.tp + (long long)cum * l.units_o + uo * nt;
+        const long long up_slot = up, uo_slot = (long long)b * l.units_o + uo;
+        float M = -INFINITY;
+        auto each = [&](auto f) {
+            if (l.lt > 0)
+                each_partial(a, l.total, tp, l.lt, up_slot,
+                             [&](long long slot) { f(a.ml_p, a.part_p, (size_t)slot * a.rows_p + rp % kM); });
+            if (nt > 0)
+                each_partial(a, l.total, to, nt, uo_slot,
+                             [&](long long slot) { f(a.ml_o, a.part_o, (size_t)slot * a.rows_o + hh % kM); });
+        };
+        each([&](const float2 *ml, const float *, size_t r) { M = fmaxf(M, __ldcg(ml + r).x); });
+        float L = 0.0f, acc[kVec];
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) acc[k] = 0.0f;
+        const bool out = blockIdx.z == 0;
+        each([&](const float2 *ml, const float *part, size_t r) {
+            const float2 x = __ldcg(ml + r);
+            const float f = ex2(x.x - M);
+            L = fmaf(x.y, f, L);
+            if (out) {
+                const float *p = part + r * C::kDV + lane * kVec;
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) acc[k] = fmaf(__ldcg(p + k), f, acc[k]);
+            }
+        });
+        const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;   // no rows: 0 (a NaN stays one)
+        if (out) {
+            T *o = static_cast<T *>(a.out) + ((size_t)b * a.n_head + (size_t)g * a.group + hh) * HD + dv * C::kDV +
+                   lane * kVec;
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) o[k] = from_f32<T>(acc[k] * inv);
+        }
+        if (dv == 0 && lane == 0) stat[hh] = make_float2(M, inv);
+    }
+    if (!a.add_weights) return;
+    __syncthreads();
+    const int n = own_len(a, b);
+    const float *sc = a.score + ((size_t)b * a.n_head + (size_t)g * a.group) * a.pitch;
+    float *w = a.row_weight + ((size_t)b * a.n_kv + g) * a.max_ctx;
+    for (int j = blockIdx.z * 32 * kCombWarps + threadIdx.x; j < n; j += gridDim.z * 32 * kCombWarps) {
+        float sum = 0.0f;
+        for (int hh = 0; hh < a.group; ++hh) {
+            const float2 x = stat[hh];
+            sum = fmaf(ex2(__ldcg(sc + (size_t)hh * a.pitch + j) - x.x), x.y, sum);
+        }
+        w[j] = a.decay == 0.0f ? sum : fmaf(a.decay, w[j], sum);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Shapes, without pointers.
 int ab_shape(const lalb_kv_batch *c, const lalb_attn_batch *p) {
     if (int st = kv_batch_shape(c)) return st;
     if (!p || p->prefix_len < 0) return LALB_ERR_INVALID;
     if (int st = lalb_attention_check(p->n_head, c->n_kv_head, c->head_dim)) return st;
-    if (p->n_head / c->n_kv_head > 1024 || (long long)p->n_head * c->head_dim > (1 << 24) || c->n_seq > 65535)
+    const long long group = p->n_head / c->n_kv_head;
+    if (group > kMaxGroup || (long long)p->n_head * c->head_dim > (1 << 24) || c->n_seq > 65535 ||
+        c->n_kv_head > 65535)
         return LALB_ERR_UNSUPPORTED;
+    // tiles of the list at most, and query rows: 31-bit indices
+    const long long mp = (c->n_seq * group + kM - 1) / kM, mo = (group + kM - 1) / kM;
+    const long long tiles = 2ll * c->n_kv_head * (mp * tiles_of(p->prefix_len) +
+                                                  mo * c->n_seq * (long long)tiles_of(c->max_ctx));
+    if (tiles > (1ll << 30) || c->n_seq * group > (1ll << 30)) return LALB_ERR_UNSUPPORTED;
     return LALB_OK;
+}
+
+constexpr int kGrid = 148;      // one CTA per SM of a B200 (workspace sizes need no device)
+
+struct Plan {
+    AbArgs a;
+    size_t o_cum, o_mlp, o_mlo, o_pp, o_po, o_score, bytes;
+};
+
+void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
+    AbArgs &a = pl->a;
+    a = AbArgs();
+    a.n_seq = c->n_seq;
+    a.n_head = p->n_head;
+    a.n_kv = c->n_kv_head;
+    a.group = p->n_head / c->n_kv_head;
+    a.hd = c->head_dim;
+    a.max_ctx = c->max_ctx;
+    a.prefix = p->prefix_len;
+    a.add_weights = p->add_weights != 0;
+    a.ndv = c->dtype == LALB_DT_F32 && c->head_dim == 256 ? 2 : 1;
+    a.m_p = (a.n_seq * a.group + kM - 1) / kM;
+    a.m_o = (a.group + kM - 1) / kM;
+    a.rows_p = std::min(kM, a.n_seq * a.group);
+    a.rows_o = std::min(kM, a.group);
+    a.grid = kGrid;
+    a.pitch = tiles_of(a.max_ctx) * kTile;
+    const int dv = a.hd / a.ndv;
+    // a segment's slot is its CTA's number plus its unit's
+    const size_t sp = a.prefix ? (size_t)kGrid + (size_t)a.n_kv * a.m_p * a.ndv : 0;
+    const size_t so = (size_t)kGrid + (size_t)a.n_seq * a.n_kv * a.m_o * a.ndv;
+    size_t off = 0;
+    auto take = [&](size_t n) {
+        const size_t at = off;
+        off += up256(n);
+        return at;
+    };
+    pl->o_cum = take(((size_t)a.n_seq + 1) * sizeof(int));
+    pl->o_mlp = take(sp * a.rows_p * sizeof(float2));
+    pl->o_mlo = take(so * a.rows_o * sizeof(float2));
+    pl->o_pp = take(sp * a.rows_p * dv * sizeof(float));
+    pl->o_po = take(so * a.rows_o * dv * sizeof(float));
+    pl->o_score = take(a.add_weights ? (size_t)a.n_seq * a.n_head * a.pitch * sizeof(float) : 0);
+    pl->bytes = off;
+}
+
+struct Kernels {
+    const void *tiles, *combine;
+    int threads, smem;
+};
+
+template <class T, int HD>
+Kernels kernels_of() {
+    using C = Cfg<T, HD>;
+    return {(const void *)attention_tiles_kernel<T, HD>, (const void *)attention_combine_kernel<T, HD>, C::kThreads,
+            (int)C::kSmem};
+}
+
+template <class T>
+Kernels kernels_for(int hd) {
+    switch (hd) {
+        case 32: return kernels_of<T, 32>();
+        case 64: return kernels_of<T, 64>();
+        case 128: return kernels_of<T, 128>();
+        default: return kernels_of<T, 256>();
+    }
 }
 
 }  // namespace
@@ -121,7 +1077,9 @@ extern "C" int lalb_attention_batch_ws_bytes(const lalb_kv_batch *cache, const l
                                              size_t *bytes) {
     if (!bytes) return LALB_ERR_INVALID;
     if (int st = ab_shape(cache, attn)) return st;
-    *bytes = 256;
+    Plan pl;
+    make_plan(cache, attn, &pl);
+    *bytes = pl.bytes;
     return LALB_OK;
 }
 
@@ -146,33 +1104,63 @@ extern "C" int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache, c
         return lalb_fail(ctx, LALB_ERR_INVALID, "attention_batch: scale and decay must be finite");
     if (attn->add_weights && !cache->row_weight)
         return lalb_fail(ctx, LALB_ERR_INVALID, "attention_batch: add_weights needs the cache's row_weight");
-    AbArgs a = {};
+    Plan pl;
+    make_plan(cache, attn, &pl);
+    AbArgs &a = pl.a;
+    uint8_t *w = static_cast<uint8_t *>(ws);
     a.q = q;
     a.pk = attn->prefix_k;
     a.pv = attn->prefix_v;
     a.k = cache->k;
     a.v = cache->v;
     a.lens = lens;
+    a.cum = reinterpret_cast<int *>(w + pl.o_cum);
+    a.ml_p = reinterpret_cast<float2 *>(w + pl.o_mlp);
+    a.ml_o = reinterpret_cast<float2 *>(w + pl.o_mlo);
+    a.part_p = reinterpret_cast<float *>(w + pl.o_pp);
+    a.part_o = reinterpret_cast<float *>(w + pl.o_po);
+    a.score = reinterpret_cast<float *>(w + pl.o_score);
     a.row_weight = cache->row_weight;
     a.out = out;
     a.status = &ctx->scratch->status;
     a.q_stride = q_stride;
-    a.n_seq = cache->n_seq;
-    a.n_head = attn->n_head;
-    a.n_kv = cache->n_kv_head;
-    a.max_ctx = cache->max_ctx;
-    a.prefix = attn->prefix_len;
-    a.add_weights = attn->add_weights;
-    a.scale = attn->scale == 0.0f ? (float)(1.0 / sqrt((double)cache->head_dim)) : attn->scale;
+    const double scale = attn->scale == 0.0f ? 1.0 / sqrt((double)cache->head_dim) : (double)attn->scale;
+    // kept away from 0, where (masked) -inf x 0 would be NaN
+    a.c = (float)std::max(1e-37, fabs(scale) * 1.4426950408889634074);
+    a.sign = scale < 0.0 ? -1.0f : 1.0f;
     a.decay = attn->decay;
     DeviceGuard guard(ctx->device);
     if (!guard.ok()) return lalb_fail(ctx, LALB_ERR_CUDA, "attention_batch: device %d", ctx->device);
-    const void *fn = cache->dtype == LALB_DT_F32   ? ab_kernel<float>(cache->head_dim)
-                     : cache->dtype == LALB_DT_F16 ? ab_kernel<__half>(cache->head_dim)
-                                                   : ab_kernel<__nv_bfloat16>(cache->head_dim);
-    void *params[] = {&a};
-    LALB_CUDA_TRY(ctx, cudaLaunchKernel(fn, dim3(cache->n_kv_head, cache->n_seq), dim3(32 * kAbWarps), params, 0,
-                                        (cudaStream_t)stream));
+    const Kernels kn = cache->dtype == LALB_DT_F32   ? kernels_for<float>(a.hd)
+                       : cache->dtype == LALB_DT_F16 ? kernels_for<__half>(a.hd)
+                                                     : kernels_for<__nv_bfloat16>(a.hd);
+    if (int st = lalb_set_smem_attr(ctx, kn.tiles, kn.smem)) return st;
+    CUtensorMap maps[4] = {};
+    if (es == 2) {
+        const CUtensorMapDataType dt =
+            cache->dtype == LALB_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        const int box = std::min(64, a.hd);
+        const CUtensorMapSwizzle sw = box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+        const void *base[4] = {a.pk, a.pv, a.k, a.v};
+        for (int i = 0; i < 4; ++i) {
+            const long long rows = i < 2 ? a.prefix : (long long)a.n_seq * a.max_ctx;
+            if (rows == 0) continue;
+            if (int st = map2d(ctx, &maps[i], base[i], dt, 2, (long long)a.n_kv * a.hd, rows, box, kTile, sw)) return st;
+        }
+    }
+    if (int st = launch_pdl(ctx, kn.tiles, dim3(a.grid), dim3(kn.threads), kn.smem, (cudaStream_t)stream,
+                            {&maps[0], &maps[1], &maps[2], &maps[3], &a}))
+        return st;
+    LALB_LAUNCH_CHECK(ctx, "attention_tiles_kernel");
+    // weights: as many CTAs per (sequence, KV head) as fill the GPU, 1024 rows each at least
+    int z = 1;
+    if (a.add_weights)
+        z = (int)std::max(1ll, std::min<long long>((a.max_ctx + 1023) / 1024,
+                                                   (4ll * ctx->sm_count) / ((long long)a.n_seq * a.n_kv)));
+    if (int st = launch_pdl(ctx, kn.combine, dim3(a.n_kv, a.n_seq, z), dim3(32 * kCombWarps), 0,
+                            (cudaStream_t)stream, {&a}))
+        return st;
+    LALB_LAUNCH_CHECK(ctx, "attention_combine_kernel");
     return LALB_OK;
 } catch (...) {   // out of host memory: no exception leaves a C entry point
     return LALB_ERR_NOMEM;
