@@ -121,26 +121,28 @@ __device__ __forceinline__ int own_len(const AbArgs &a, int b) {
     return n < 0 || n > a.max_ctx ? 0 : n;
 }
 
-// The tile list: prefix tiles first, then per sequence its units.
+// The tile list: prefix tiles first, then per sequence its units.  CTA c takes
+// `per` tiles, the first `rem` CTAs one more.  (The host bounds every index.)
 struct List {
-    long long tp, total;   // prefix tiles, all tiles
+    int tp, total;         // prefix tiles, all tiles
     int lt;                // tiles of a prefix unit
     int units_o;           // own units per sequence
+    int per, rem;
+
+    __device__ __forceinline__ List(const AbArgs &a, int own_tiles) {
+        lt = tiles_of(a.prefix);
+        tp = a.n_kv * a.m_p * a.ndv * lt;
+        units_o = a.n_kv * a.m_o * a.ndv;
+        total = tp + own_tiles * units_o;
+        per = total / a.grid;
+        rem = total - per * a.grid;
+    }
+    __device__ __forceinline__ int first(int c) const { return c * per + min(c, rem); }
+    __device__ __forceinline__ int owner(int t) const {
+        const int big = (per + 1) * rem;
+        return t < big ? t / (per + 1) : rem + (t - big) / per;
+    }
 };
-
-__device__ __forceinline__ List make_list(const AbArgs &a, long long own_tiles) {
-    List l;
-    l.lt = tiles_of(a.prefix);
-    l.tp = (long long)a.n_kv * a.m_p * a.ndv * l.lt;
-    l.units_o = a.n_kv * a.m_o * a.ndv;
-    l.total = l.tp + own_tiles * l.units_o;
-    return l;
-}
-
-__device__ __forceinline__ long long cta_first(long long total, int grid, int c) {
-    return (total * c + grid - 1) / grid;
-}
-__device__ __forceinline__ int cta_of(long long total, int grid, long long t) { return (int)(t * grid / total); }
 
 struct Seg {
     bool prefix;
@@ -149,48 +151,49 @@ struct Seg {
     int j0, j1;            // tiles of the unit
     int n;                 // rows of the unit's cache
     int rows;              // query rows of the unit
-    long long slot;        // partial
+    int slot;              // partial
 };
 
 // Walks one CTA's segments.  Every role walks on its own.
 struct Walk {
-    long long t, end;
+    int t, end;
     int b;
-    long long c0;          // list position of sequence b's first own tile, less tp
+    int c0;                // list position of sequence b's first own tile, less tp
     int n, nt;             // length and tiles of sequence b
 
     __device__ __forceinline__ bool next(const AbArgs &a, const List &l, Seg &s) {
         if (t >= end) return false;
         int u, units;
         if (t < l.tp) {
-            u = (int)(t / l.lt);
+            u = t / l.lt;
             s.prefix = true;
-            s.j0 = (int)(t % l.lt);
-            s.j1 = (int)min((long long)l.lt, s.j0 + (min(end, l.tp) - t));
+            s.j0 = t - u * l.lt;
+            s.j1 = min(l.lt, s.j0 + (min(end, l.tp) - t));
             s.n = a.prefix;
-            s.slot = (long long)blockIdx.x + u;
+            s.slot = blockIdx.x + u;
             units = a.m_p;
             s.b = 0;
         } else {
-            const long long o = t - l.tp;
-            while (o >= c0 + (long long)nt * l.units_o) {
-                c0 += (long long)nt * l.units_o;
+            const int o = t - l.tp;
+            while (o >= c0 + nt * l.units_o) {
+                c0 += nt * l.units_o;
                 ++b;
                 n = own_len(a, b);
                 nt = tiles_of(n);
             }
-            u = (int)((o - c0) / nt);
+            u = (o - c0) / nt;
             s.prefix = false;
-            s.j0 = (int)((o - c0) % nt);
-            s.j1 = (int)min((long long)nt, s.j0 + (end - t));
+            s.j0 = o - c0 - u * nt;
+            s.j1 = min(nt, s.j0 + (end - t));
             s.n = n;
-            s.slot = (long long)blockIdx.x + (long long)b * l.units_o + u;
+            s.slot = blockIdx.x + b * l.units_o + u;
             units = a.m_o;
             s.b = b;
         }
-        s.dv = u % a.ndv;
-        s.m = u / a.ndv % units;
-        s.g = u / a.ndv / units;
+        const int v = u / a.ndv;
+        s.dv = u - v * a.ndv;
+        s.g = v / units;
+        s.m = v - s.g * units;
         s.rows = min(kM, (s.prefix ? a.n_seq * a.group : a.group) - s.m * kM);
         t += s.j1 - s.j0;
         return true;
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     uint64_t *qready = ofull + 2;              // Q of the segment written, O of the last one read
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(qready + 1);
     int *start_b = reinterpret_cast<int *>(tmem_slot + 1);
-    long long *start = reinterpret_cast<long long *>(start_b + 1);    // own tiles of all, of those before start_b
+    int *start = start_b + 1;                  // own tiles of all, of those before start_b, start_b's length
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     pdl_wait();
     // ---- the list: its length, and where this CTA's own tiles begin ---------------------
     if (warp == 0) {
-        long long sum = 0;
+        int sum = 0;
         for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
             const int b = b0 + lane;
             int nt = 0;
@@ -397,18 +400,17 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 const int x = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += x;
             }
-            if (blockIdx.x == 0 && b < a.n_seq) a.cum[b] = (int)sum + incl - nt;
+            if (blockIdx.x == 0 && b < a.n_seq) a.cum[b] = sum + incl - nt;
             sum += __shfl_sync(0xffffffffu, incl, 31);
         }
-        if (blockIdx.x == 0 && lane == 0) a.cum[a.n_seq] = (int)sum;
-        const List l = make_list(a, sum);
-        const long long first = cta_first(l.total, a.grid, blockIdx.x) - l.tp;   // among the own tiles
+        if (blockIdx.x == 0 && lane == 0) a.cum[a.n_seq] = sum;
+        const List l(a, sum);
+        const int first = l.first(blockIdx.x) - l.tp;   // among the own tiles
         // the sequence of that tile (of the first one, if the CTA begins in the prefix)
-        int sb = 0;
-        long long before = 0;
+        int sb = 0, before = 0;
         if (first > 0 && first < sum * l.units_o) {
-            const long long want = first / l.units_o;     // cum[sb] <= want < cum[sb + 1]
-            long long run = 0;
+            const int want = first / l.units_o;     // cum[sb] <= want < cum[sb + 1]
+            int run = 0;
             for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
                 const int b = b0 + lane;
                 const int nt = b < a.n_seq ? tiles_of(own_len(a, b)) : 0;
@@ -432,6 +434,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             *start_b = sb;
             start[0] = sum;
             start[1] = before;
+            start[2] = own_len(a, sb);
         }
     }
     __syncthreads();
@@ -442,13 +445,13 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     // raises a status bit and skips the work
     const bool tmem_ok = tmem == 0;
     if (!tmem_ok && threadIdx.x == 0) atomicOr(a.status, LALB_STATUS_WAIT_TIMEOUT);
-    const List list = make_list(a, start[0]);
+    const List list(a, start[0]);
     Walk walk;
-    walk.t = list.total ? cta_first(list.total, a.grid, blockIdx.x) : 0;
-    walk.end = list.total && tmem_ok ? cta_first(list.total, a.grid, blockIdx.x + 1) : 0;
+    walk.t = list.first(blockIdx.x);
+    walk.end = tmem_ok ? list.first(blockIdx.x + 1) : 0;
     walk.b = *start_b;
     walk.c0 = start[1] * list.units_o;
-    walk.n = own_len(a, walk.b);
+    walk.n = start[2];
     walk.nt = tiles_of(walk.n);
     Seg s;
 
@@ -904,18 +907,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
 
 // ---- the rows' partials together, and the rows' weights -----------------------------------------
 constexpr int kCombWarps = 8;
+constexpr int kCombUnroll = 8;        // partials of a row in flight
 constexpr int kMaxGroup = 1024;
-
-// Runs over the partials of one unit: tiles [t, t + nt) of the list.
-template <class F>
-__device__ __forceinline__ void each_partial(const AbArgs &a, long long total, long long t, int nt, long long unit,
-                                             F f) {
-    const int c0 = cta_of(total, a.grid, t), c1 = cta_of(total, a.grid, t + nt - 1);
-    for (int c = c0; c <= c1; ++c) {
-        // a CTA between them may have no tile at all
-        if (cta_first(total, a.grid, c) < cta_first(total, a.grid, c + 1)) f(c + unit);
-    }
-}
 
 // CTA (KV head g, sequence b, z): warps take the group's heads; z = 0 writes
 // the outputs, and all z share the rows whose weights are kept.
@@ -928,45 +921,72 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
     pdl_wait();
     pdl_launch_dependents();
     const int cum = __ldcg(a.cum + b), nt = __ldcg(a.cum + b + 1) - cum;
-    const List l = make_list(a, __ldcg(a.cum + a.n_seq));
+    const List l(a, __ldcg(a.cum + a.n_seq));
     const int n_out = blockIdx.z == 0 ? C::kNDV : 1;    // the weights need one half's sums only
+    const bool out = blockIdx.z == 0;
     for (int i = warp; i < a.group * n_out; i += kCombWarps) {
         const int hh = i / n_out, dv = i % n_out;
+        // the row's partials: a unit's are its CTAs' in turn, `np` prefix ones first
         const int rp = b * a.group + hh;
-        const long long up = ((long long)g * a.m_p + rp / kM) * a.ndv + dv;
-        const long long uo = ((long long)g * a.m_o + hh / kM) * a.ndv + dv;
-        const long long tp = up * l.lt, to = l.tp + (long long)cum * l.units_o + uo * nt;
-        const long long up_slot = up, uo_slot = (long long)b * l.units_o + uo;
-        float M = -INFINITY;
-        auto each = [&](auto f) {
-            if (l.lt > 0)
-                each_partial(a, l.total, tp, l.lt, up_slot,
-                             [&](long long slot) { f(a.ml_p, a.part_p, (size_t)slot * a.rows_p + rp % kM); });
-            if (nt > 0)
-                each_partial(a, l.total, to, nt, uo_slot,
-                             [&](long long slot) { f(a.ml_o, a.part_o, (size_t)slot * a.rows_o + hh % kM); });
-        };
-        each([&](const float2 *ml, const float *, size_t r) { M = fmaxf(M, __ldcg(ml + r).x); });
-        float L = 0.0f, acc[kVec];
+        const int up = (g * a.m_p + rp / kM) * C::kNDV + dv, uo = (g * a.m_o + hh / kM) * C::kNDV + dv;
+        int np = 0, no = 0, cp = 0, co = 0;
+        if (l.lt > 0) {
+            cp = l.owner(up * l.lt);
+            np = l.owner(up * l.lt + l.lt - 1) - cp + 1;
+        }
+        if (nt > 0) {
+            const int to = l.tp + cum * l.units_o + uo * nt;
+            co = l.owner(to);
+            no = l.owner(to + nt - 1) - co + 1;
+        }
+        const size_t r0p = (size_t)(cp + up) * a.rows_p + rp % kM;
+        const size_t r0o = (size_t)(co + b * l.units_o + uo) * a.rows_o + hh % kM;
+        float M = -INFINITY, L = 0.0f, acc[kVec];
 #pragma unroll
         for (int k = 0; k < kVec; ++k) acc[k] = 0.0f;
-        const bool out = blockIdx.z == 0;
-        each([&](const float2 *ml, const float *part, size_t r) {
-            const float2 x = __ldcg(ml + r);
-            const float f = ex2(x.x - M);
-            L = fmaf(x.y, f, L);
-            if (out) {
-                const float *p = part + r * C::kDV + lane * kVec;
+        for (int k0 = 0; k0 < np + no; k0 += 32) {
+            const int k = k0 + lane;
+            float2 x = make_float2(-INFINITY, 0.0f);
+            if (k < np)
+                x = __ldcg(a.ml_p + r0p + (size_t)k * a.rows_p);
+            else if (k < np + no)
+                x = __ldcg(a.ml_o + r0o + (size_t)(k - np) * a.rows_o);
+            float top = x.x;
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) acc[k] = fmaf(__ldcg(p + k), f, acc[k]);
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(M, top);
+            const float f = k < np + no ? ex2(x.x - top) : 0.0f, old = k0 ? ex2(M - top) : 0.0f;
+            M = top;
+            L = fmaf(L, old, warp_sum(x.y * f));
+            if (!out) continue;
+#pragma unroll
+            for (int q = 0; q < kVec; ++q) acc[q] *= old;
+            const int m = min(32, np + no - k0);
+#pragma unroll 1
+            for (int j0 = 0; j0 < m; j0 += kCombUnroll) {
+                float v[kCombUnroll][kVec];
+#pragma unroll
+                for (int j = 0; j < kCombUnroll; ++j) {
+                    const int kk = k0 + j0 + j;
+                    const float *p = kk < np ? a.part_p + (r0p + (size_t)kk * a.rows_p) * C::kDV
+                                             : a.part_o + (r0o + (size_t)(kk - np) * a.rows_o) * C::kDV;
+#pragma unroll
+                    for (int q = 0; q < kVec; ++q) v[j][q] = j0 + j < m ? __ldcg(p + lane + 32 * q) : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < kCombUnroll; ++j) {
+                    const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
+#pragma unroll
+                    for (int q = 0; q < kVec; ++q) acc[q] = fmaf(v[j][q], w, acc[q]);
+                }
             }
-        });
+        }
         const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;   // no rows: 0 (a NaN stays one)
         if (out) {
             T *o = static_cast<T *>(a.out) + ((size_t)b * a.n_head + (size_t)g * a.group + hh) * HD + dv * C::kDV +
-                   lane * kVec;
+                   lane;
 #pragma unroll
-            for (int k = 0; k < kVec; ++k) o[k] = from_f32<T>(acc[k] * inv);
+            for (int k = 0; k < kVec; ++k) o[32 * k] = from_f32<T>(acc[k] * inv);
         }
         if (dv == 0 && lane == 0) stat[hh] = make_float2(M, inv);
     }
