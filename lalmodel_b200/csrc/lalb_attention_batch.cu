@@ -55,6 +55,7 @@ using namespace lalb;
 
 namespace {
 
+constexpr int kGrid = 148;           // one CTA per SM of a B200 (workspace sizes need no device)
 constexpr int kTile = 64;            // cache rows per tile
 constexpr int kM = 128;              // query rows per unit
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (loaders run at most 5 ahead)
@@ -75,11 +76,19 @@ struct Cfg {
     static constexpr int kColO = 512 - kNS * kDV;
     static_assert(kColQ + kQCols <= kColO, "Q and O fit TMEM");
     static constexpr int kSoftWarps = 4 * kNS;
-    // F32: 7, so that a block of two softmax warpgroups, the MMA warp and the
-    // loaders has 16 warps and 128 registers a thread
+    // F32: 7, which with the MMA warp makes two warpgroups
     static constexpr int kLoadWarps = kF32 ? 7 : 1;
     static constexpr int kFullCount = kF32 ? 8 : 1;    // arrivals that fill a stage: its groups of 8 rows
-    static constexpr int kThreads = 32 * (kSoftWarps + 1 + kLoadWarps);
+    static constexpr int kOtherWarps = kF32 ? 8 : 4;   // MMA, loaders (16 bits: two warps idle)
+    static constexpr int kThreads = 32 * (kSoftWarps + kOtherWarps);
+    // Registers a thread: the launch's even share, and the split of it (the
+    // softmax holds a tile's scores and weights; at the even share it spills)
+    static constexpr int kEven = kThreads == 512 ? 128 : kThreads == 384 ? 168 : 248;
+    static constexpr int kSoftRegs = kF32 ? (kNS == 2 ? 152 : 232) : kNS == 2 ? 216 : 0;   // 0: no split
+    static constexpr int kOtherRegs = kF32 ? (kNS == 2 ? 104 : 136) : 72;
+    static_assert(kSoftRegs == 0 || kSoftRegs * kSoftWarps + kOtherRegs * kOtherWarps <=
+                                        kEven * (kSoftWarps + kOtherWarps),
+                  "the split is no more than the block was launched with");
     static constexpr uint32_t kStage = kTile * HD * (kF32 ? 4 : 2);
     static constexpr int kBudget = kNS == 2 ? kStageBudget2 : kStageBudget1;
     static constexpr int kStages = kBudget / (int)kStage < 10 ? kBudget / (int)kStage : 10;
@@ -89,7 +98,7 @@ struct Cfg {
     static constexpr uint32_t kSub = kTile * kSubW * 2;               // its bytes
     static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
     static constexpr uint32_t kOffMl = kOffScratch + kSoftWarps * 4096;
-    static constexpr uint32_t kOffSide = kOffMl + 2 * kM * 8;
+    static constexpr uint32_t kOffSide = kOffMl + 2 * kM * 8 + (kF32 ? 2 * kM * 4 : 0);   // ml, and F32's qmax
     static constexpr uint32_t kOffBar = kOffSide + kSide * 16 * 4;
     static constexpr uint32_t kSmem = 1024 + kOffBar + 512;
     static_assert(kSmem <= 232448, "fits the 227 KB opt-in shared memory");
@@ -110,7 +119,7 @@ struct AbArgs {
     int n_seq, n_head, n_kv, group, hd, max_ctx, prefix, add_weights;
     int m_p, m_o;                // 128-row tiles of a prefix and an own unit's KV head
     int rows_p, rows_o;          // rows kept per partial
-    int ndv, grid, pitch;
+    int pitch;
     float c, decay, sign;        // |scale| log2 e, sign of the scale
 };
 
@@ -129,13 +138,13 @@ struct List {
     int units_o;           // own units per sequence
     int per, rem;
 
-    __device__ __forceinline__ List(const AbArgs &a, int own_tiles) {
+    __device__ __forceinline__ List(const AbArgs &a, int ndv, int own_tiles) {
         lt = tiles_of(a.prefix);
-        tp = a.n_kv * a.m_p * a.ndv * lt;
-        units_o = a.n_kv * a.m_o * a.ndv;
+        tp = a.n_kv * a.m_p * ndv * lt;
+        units_o = a.n_kv * a.m_o * ndv;
         total = tp + own_tiles * units_o;
-        per = total / a.grid;
-        rem = total - per * a.grid;
+        per = total / kGrid;
+        rem = total - per * kGrid;
     }
     __device__ __forceinline__ int first(int c) const { return c * per + min(c, rem); }
     __device__ __forceinline__ int owner(int t) const {
@@ -161,6 +170,7 @@ struct Walk {
     int c0;                // list position of sequence b's first own tile, less tp
     int n, nt;             // length and tiles of sequence b
 
+    template <int NDV>
     __device__ __forceinline__ bool next(const AbArgs &a, const List &l, Seg &s) {
         if (t >= end) return false;
         int u, units;
@@ -190,9 +200,9 @@ struct Walk {
             units = a.m_o;
             s.b = b;
         }
-        const int v = u / a.ndv;
-        s.dv = u - v * a.ndv;
-        s.g = v / units;
+        const int v = u / NDV;
+        s.dv = u - v * NDV;
+        s.g = units == 1 ? v : v / units;
         s.m = v - s.g * units;
         s.rows = min(kM, (s.prefix ? a.n_seq * a.group : a.group) - s.m * kM);
         t += s.j1 - s.j0;
@@ -217,6 +227,14 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, float *r) {
           "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, float *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -230,6 +248,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+
+// A warpgroup's registers from here on (0: as launched).  In the role's own
+// branch: where roles meet again the compiler keeps to the smaller share.
+template <int N, bool INC>
+__device__ __forceinline__ void set_regs() {
+    if constexpr (N != 0 && INC)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N) : "memory");
+    else if constexpr (N != 0)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N) : "memory");
 }
 
 template <class T>
@@ -353,8 +381,9 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     uint64_t *sfull = empty + C::kStages;      // S(j) complete (and every product before it)
     uint64_t *pready = sfull + 2;              // P(j) written
     uint64_t *ofull = pready + 2;              // a stream's latest PV complete
-    uint64_t *qready = ofull + 2;              // Q of the segment written, O of the last one read
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(qready + 1);
+    uint64_t *qready = ofull + 2;              // Q of the segment written
+    uint64_t *oready = qready + 1;             // O of the segment read
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(oready + 1);
     int *start_b = reinterpret_cast<int *>(tmem_slot + 1);
     int *start = start_b + 1;                  // own tiles of all, of those before start_b, start_b's length
 
@@ -370,6 +399,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             mbar_init(&ofull[s], 1);
         }
         mbar_init(qready, C::kSoftWarps);
+        mbar_init(oready, C::kSoftWarps);
         fence_barrier_init();
     }
     if (warp == C::kSoftWarps) {
@@ -382,59 +412,66 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     pdl_wait();
     // ---- the list: its length, and where this CTA's own tiles begin ---------------------
     if (warp == 0) {
-        int sum = 0;
-        for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-            const int b = b0 + lane;
-            int nt = 0;
-            if (b < a.n_seq) {
-                const int n = __ldcg(a.lens + b);
-                if (n < 0 || n > a.max_ctx) {
-                    if (blockIdx.x == 0) atomicOr(a.status, LALB_STATUS_BAD_POSITION);
-                } else {
-                    nt = tiles_of(n);
-                }
-            }
-            int incl = nt;
+        // tiles of 32 sequences at a time, the first kHold x 32 of them loaded
+        // together and kept for the second look
+        constexpr int kHold = 8;
+        int held[kHold];
+        auto length = [&](int b) { return b < a.n_seq ? __ldcg(a.lens + b) : 0; };
+        auto tiles = [&](int n) { return n < 0 || n > a.max_ctx ? 0 : tiles_of(n); };
+        auto scan = [&](int x) {
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += x;
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
             }
-            if (blockIdx.x == 0 && b < a.n_seq) a.cum[b] = sum + incl - nt;
-            sum += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (blockIdx.x == 0 && lane == 0) a.cum[a.n_seq] = sum;
-        const List l(a, sum);
-        const int first = l.first(blockIdx.x) - l.tp;   // among the own tiles
-        // the sequence of that tile (of the first one, if the CTA begins in the prefix)
-        int sb = 0, before = 0;
-        if (first > 0 && first < sum * l.units_o) {
-            const int want = first / l.units_o;     // cum[sb] <= want < cum[sb + 1]
-            int run = 0;
-            for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-                const int b = b0 + lane;
-                const int nt = b < a.n_seq ? tiles_of(own_len(a, b)) : 0;
-                int incl = nt;
+            return x;
+        };
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int x = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += x;
-                }
+        for (int i = 0; i < kHold; ++i) held[i] = length(32 * i + lane);
+        int sum = 0;
+        auto look = [&](int b0, int n) {
+            if (n < 0 || n > a.max_ctx) {
+                if (blockIdx.x == 0) atomicOr(a.status, LALB_STATUS_BAD_POSITION);
+            }
+            const int incl = scan(tiles(n));
+            if (blockIdx.x == 0 && b0 + lane < a.n_seq) a.cum[b0 + lane] = sum + incl - tiles(n);
+            sum += __shfl_sync(0xffffffffu, incl, 31);
+        };
+#pragma unroll
+        for (int i = 0; i < kHold; ++i)
+            if (32 * i < a.n_seq) look(32 * i, held[i]);
+        for (int b0 = 32 * kHold; b0 < a.n_seq; b0 += 32) look(b0, length(b0 + lane));
+        if (blockIdx.x == 0 && lane == 0) a.cum[a.n_seq] = sum;
+        const List l(a, C::kNDV, sum);
+        const int first = l.first(blockIdx.x) - l.tp;   // among the own tiles
+        // the sequence of that tile (the first one, if the CTA begins in the prefix)
+        const int want = first > 0 ? first / l.units_o : 0;
+        int sb = 0, before = 0, n0 = __shfl_sync(0xffffffffu, held[0], 0);
+        if (first > 0 && first < sum * l.units_o) {     // cum[sb] <= want < cum[sb + 1]
+            int run = 0;
+            bool found = false;
+            auto find = [&](int b0, int n) {
+                const int nt = tiles(n), incl = scan(nt);
                 const uint32_t past = __ballot_sync(0xffffffffu, run + incl > want);
                 if (past) {
                     const int i = __ffs(past) - 1;
                     sb = b0 + i;
                     before = run + __shfl_sync(0xffffffffu, incl - nt, i);
-                    break;
+                    n0 = __shfl_sync(0xffffffffu, n, i);
+                    found = true;
                 }
                 run += __shfl_sync(0xffffffffu, incl, 31);
-            }
+            };
+#pragma unroll
+            for (int i = 0; i < kHold; ++i)
+                if (!found && 32 * i < a.n_seq) find(32 * i, held[i]);
+            for (int b0 = 32 * kHold; !found && b0 < a.n_seq; b0 += 32) find(b0, length(b0 + lane));
         }
         if (lane == 0) {
             *start_b = sb;
             start[0] = sum;
             start[1] = before;
-            start[2] = own_len(a, sb);
+            start[2] = n0 < 0 || n0 > a.max_ctx ? 0 : n0;
         }
     }
     __syncthreads();
@@ -445,7 +482,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     // raises a status bit and skips the work
     const bool tmem_ok = tmem == 0;
     if (!tmem_ok && threadIdx.x == 0) atomicOr(a.status, LALB_STATUS_WAIT_TIMEOUT);
-    const List list(a, start[0]);
+    const List list(a, C::kNDV, start[0]);
     Walk walk;
     walk.t = list.first(blockIdx.x);
     walk.end = tmem_ok ? list.first(blockIdx.x + 1) : 0;
@@ -455,7 +492,10 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     walk.nt = tiles_of(walk.n);
     Seg s;
 
-    if (warp > C::kSoftWarps) {
+    if (warp > C::kSoftWarps + C::kLoadWarps) {
+        set_regs<C::kSoftRegs ? C::kOtherRegs : 0, false>();     // idle
+    } else if (warp > C::kSoftWarps) {
+        set_regs<C::kSoftRegs ? C::kOtherRegs : 0, false>();
         // ================================ loaders ===============================================
         if constexpr (C::kF32) {
             // a stage is 8 groups of 8 rows; the groups go round the loader warps
@@ -479,7 +519,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[slot]);
             };
-            while (walk.next(a, list, s)) {
+            while (walk.template next<C::kNDV>(a, list, s)) {
                 const size_t seq = s.prefix ? 0 : (size_t)s.b * a.max_ctx * pitch;
                 const float *kb = static_cast<const float *>(s.prefix ? a.pk : a.k) + seq + (size_t)s.g * HD;
                 const float *vb =
@@ -504,7 +544,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         } else if (lane == 0) {
             uint32_t st = 0;
             bool ok = true;
-            while (walk.next(a, list, s)) {
+            while (walk.template next<C::kNDV>(a, list, s)) {
                 const CUtensorMap *mk = s.prefix ? &mPK : &mK, *mv = s.prefix ? &mPV : &mV;
                 const int row0 = s.prefix ? 0 : s.b * a.max_ctx;
                 for (int j = s.j0; j < s.j1 && ok; ++j)
@@ -527,6 +567,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         }
     } else if (warp == C::kSoftWarps) {
         // ================================ MMA ====================================================
+        set_regs<C::kSoftRegs ? C::kOtherRegs : 0, false>();
         constexpr uint32_t kIdS = mma_idesc<typename std::conditional<C::kF32, __half, T>::type>(kTile, false);
         constexpr uint32_t kIdO = mma_idesc<typename std::conditional<C::kF32, __half, T>::type>(C::kDV, true);
         constexpr uint32_t kLoK = kTile * HD * 2, kLoV = kTile * C::kDV * 2;
@@ -559,7 +600,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             commit_elect(&ofull[stream]);
             return true;
         };
-        while (ok && walk.next(a, list, s)) {
+        while (ok && walk.template next<C::kNDV>(a, list, s)) {
             if (!(ok = warp_wait_fast(qready, segs & 1u, a.status))) break;
             tc_after();
             ++segs;
@@ -594,6 +635,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     // tile i - 1's values: the stage before K(i) (the last one: before the end)
                     const uint32_t v = vslot;
                     const bool first = i - 1 < C::kNS;
+                    // the last segment's O is read by now, or will be soon
+                    if (i == 1 && segs > 1 && !(ok = warp_wait_fast(oready, segs & 1u, a.status))) break;
                     if (!(ok = issue_pv(tile + i - 1, v % C::kStages, v / C::kStages, first))) break;
                 }
                 vslot = st + 1;
@@ -603,83 +646,147 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         }
     } else {
         // ================================ softmax ==================================================
+        set_regs<C::kSoftRegs, true>();
         const int wg = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         uint8_t *scratch = smem + C::kOffScratch + warp * 4096;
+        float *qmax = reinterpret_cast<float *>(ml + 2 * kM);   // F32: [warpgroup][row] largest |q| of its columns
         uint32_t tile = 0, st = 0;              // before the segment
-        uint32_t pv[2] = {0, 0};                // products of each stream so far
+        uint32_t pv0 = 0, pv1 = 0;              // products of each stream so far
         bool ok = true;
         auto soft_bar = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kSoftWarps) : "memory"); };
-        while (walk.next(a, list, s)) {
-            const int n = s.j1 - s.j0;
-            const bool active = quarter * 32 < s.rows;    // a row of this warp belongs to the unit
-            const bool mine = row < s.rows;
-            // ---- Q: this warp's rows, the columns of its warpgroup, into TMEM ------------------
-            float cq = a.c;                               // score factor of this thread's row
-            if (active) {
-                const T *qb = static_cast<const T *>(a.q) + (size_t)s.g * a.group * HD;
-                auto q_row = [&](int r) -> const T * {    // query row r of the unit
-                    const int rr = s.m * kM + r;
-                    const int b = s.prefix ? rr / a.group : s.b, h = s.prefix ? rr % a.group : rr;
-                    return qb + (size_t)b * a.q_stride + (size_t)h * HD;
-                };
-                constexpr int kLpr = 2 * sizeof(T);       // lanes per row of a 32-column chunk
-                constexpr int kRpi = 32 / kLpr;
-                const int lr = lane / kLpr, lu = lane % kLpr;
-                const int live = min(32, s.rows - quarter * 32);
-                float qs = a.sign;
-                if constexpr (C::kF32) {
-                    // the row's largest value, by the lanes that read it side by side
-                    float mine_max = 0.0f;
-                    for (int r = 0; r < live; r += kRpi) {
-                        float m = 0.0f;
-                        if (r + lr < live) {
-                            const float *p = reinterpret_cast<const float *>(q_row(quarter * 32 + r + lr)) + lu * 4;
+
+        // ---- Q: this warp's 32 rows, the 32-column chunks of its warpgroup, into TMEM ----------------
+        // Loaded kLpr lanes to a row (whole sectors), turned to a row per lane in
+        // the warp's scratch memory.  A batch is what the registers hold.
+        constexpr int kLpr = 2 * sizeof(T), kRpi = 32 / kLpr, kIt = 32 / kRpi;   // lanes per row, rows per load
+        constexpr int kChunks = HD / 32 < C::kNS ? 1 : HD / 32 / C::kNS;        // of this warpgroup
+        const bool q_idle = wg >= HD / 32;      // head_dim 32: one chunk, the first warpgroup's
+        constexpr int kBatch = 16 / kIt < kChunks ? 16 / kIt : kChunks;         // chunks per batch
+        const int lr = lane / kLpr, lu = lane % kLpr;
+        auto q_load = [&](const Seg &g, int c0, uint4 (&v)[kBatch * kIt]) {
+            const T *qb = static_cast<const T *>(a.q) + (size_t)g.g * a.group * HD + (c0 * C::kNS + wg) * 32;
+            // row r of the unit: head h of sequence b, and kRpi rows further each time
+            int r = quarter * 32 + lr, b = g.b, h = g.m * kM + r;
+            if (g.prefix) {
+                b = h / a.group;
+                h -= b * a.group;
+            }
 #pragma unroll
-                            for (int c = 0; c < HD / 32; ++c) {
-                                const float4 v = __ldg(reinterpret_cast<const float4 *>(p + 32 * c));
-                                m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-                            }
-                        }
+            for (int i = 0; i < kIt; ++i) {
+                const T *p = qb + (size_t)b * a.q_stride + (size_t)h * HD;
 #pragma unroll
-                        for (int o = 1; o < kLpr; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        const float x = __shfl_sync(0xffffffffu, m, ((lane - r) & (kRpi - 1)) * kLpr);
-                        if (lane >= r && lane < r + kRpi) mine_max = x;
+                for (int c = 0; c < kBatch; ++c)
+                    v[c * kIt + i] = r < g.rows ? __ldg(reinterpret_cast<const uint4 *>(p + c * C::kNS * 32) + lu)
+                                                : make_uint4(0, 0, 0, 0);
+                r += kRpi;
+                h += kRpi;
+                if (g.prefix)
+                    while (h >= a.group) h -= a.group, ++b;
+            }
+        };
+        // F32: the rows' largest |q| in a batch, for the lane that owns the row
+        auto q_top = [&](const uint4 (&v)[kBatch * kIt], float top) {
+#pragma unroll
+            for (int i = 0; i < kIt; ++i) {
+                float m = 0.0f;
+#pragma unroll
+                for (int c = 0; c < kBatch; ++c) {
+                    const uint4 x = v[c * kIt + i];
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(__uint_as_float(x.x)), fabsf(__uint_as_float(x.y))),
+                                       fmaxf(fabsf(__uint_as_float(x.z)), fabsf(__uint_as_float(x.w)))));
+                }
+#pragma unroll
+                for (int o = 1; o < kLpr; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const float x = __shfl_sync(0xffffffffu, m, (lane % kRpi) * kLpr);
+                if (lane / kRpi == i) top = fmaxf(top, x);
+            }
+            return top;
+        };
+        auto q_store = [&](int c0, const uint4 (&v)[kBatch * kIt], float qs) {
+#pragma unroll
+            for (int c = 0; c < kBatch; ++c) {
+#pragma unroll
+                for (int i = 0; i < kIt; ++i) {
+                    const int r = i * kRpi + lr;
+                    *reinterpret_cast<uint4 *>(scratch + r * 128 + ((lu ^ (r & 7)) << 4)) = v[c * kIt + i];
+                }
+                __syncwarp();
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int u = 0; u < kLpr; ++u) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4));
+                    if constexpr (C::kF32) {
+                        hi[2 * u] = split2<__half>(__uint_as_float(x.x) * qs, __uint_as_float(x.y) * qs, lo[2 * u]);
+                        hi[2 * u + 1] =
+                            split2<__half>(__uint_as_float(x.z) * qs, __uint_as_float(x.w) * qs, lo[2 * u + 1]);
+                    } else {
+                        // a negative scale turns the queries' signs
+                        const uint32_t f = qs < 0.0f ? 0x80008000u : 0u;
+                        hi[4 * u] = x.x ^ f, hi[4 * u + 1] = x.y ^ f, hi[4 * u + 2] = x.z ^ f, hi[4 * u + 3] = x.w ^ f;
                     }
-                    const int e = part_exponent(mine_max);
+                }
+                const uint32_t col = lanes + kColQ + 16 * ((c0 + c) * C::kNS + wg);
+                tmem_st16(col, hi);
+                if constexpr (C::kF32) tmem_st16(col + HD / 2, lo);
+                __syncwarp();
+            }
+        };
+        uint4 qv[kBatch * kIt];
+        // before the barrier both warpgroups pass at a segment's start ..
+        auto q_begin = [&](const Seg &g) {
+            if (quarter * 32 >= g.rows || q_idle) return;
+            q_load(g, 0, qv);
+        };
+        auto q_share = [&](const Seg &g) {
+            if constexpr (C::kF32) {
+                if (quarter * 32 >= g.rows || q_idle) return;
+                float top = q_top(qv, 0.0f);
+                for (int c = kBatch; c < kChunks; c += kBatch) {
+                    uint4 v[kBatch * kIt];
+                    q_load(g, c, v);
+                    top = q_top(v, top);
+                }
+                qmax[wg * kM + row] = top;
+            }
+        };
+        // .. and after it: Q written, the score factor of this thread's row returned
+        auto q_finish = [&](const Seg &g) -> float {
+            float qs = a.sign, cq = a.c;
+            if (quarter * 32 < g.rows) {
+                if constexpr (C::kF32) {
+                    const float top = C::kNS == 2 && HD > 32 ? fmaxf(qmax[row], qmax[kM + row]) : qmax[row];
+                    const int e = part_exponent(top);
                     qs = a.sign * pow2(-e);
                     cq = a.c * pow2(e);
                 }
-                for (int c = wg; c < HD / 32; c += C::kNS) {
-                    for (int r = 0; r < live; r += kRpi)
-                        if (r + lr < live) {
-                            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(q_row(quarter * 32 + r + lr) + 32 * c) + lu);
-                            *reinterpret_cast<uint4 *>(scratch + (r + lr) * 128 + ((lu ^ ((r + lr) & 7)) << 4)) = v;
-                        }
-                    __syncwarp();
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int u = 0; u < kLpr; ++u) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4));
-                        if constexpr (C::kF32) {
-                            hi[2 * u] = split2<__half>(__uint_as_float(v.x) * qs, __uint_as_float(v.y) * qs, lo[2 * u]);
-                            hi[2 * u + 1] = split2<__half>(__uint_as_float(v.z) * qs, __uint_as_float(v.w) * qs, lo[2 * u + 1]);
-                        } else {
-                            // a negative scale turns the queries' signs
-                            const uint32_t f = qs < 0.0f ? 0x80008000u : 0u;
-                            hi[4 * u] = v.x ^ f, hi[4 * u + 1] = v.y ^ f, hi[4 * u + 2] = v.z ^ f, hi[4 * u + 3] = v.w ^ f;
-                        }
-                    }
-                    tmem_st16(lanes + kColQ + 16 * c, hi);
-                    if constexpr (C::kF32) tmem_st16(lanes + kColQ + HD / 2 + 16 * c, lo);
-                    __syncwarp();
+                if (!q_idle) q_store(0, qv, qs);
+                for (int c = kBatch; c < kChunks; c += kBatch) {
+                    uint4 v[kBatch * kIt];
+                    q_load(g, c, v);
+                    q_store(c, v, qs);
                 }
                 tmem_wait_st();
             }
             tc_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(qready);
+            return cq;
+        };
 
+        Seg nx;
+        bool have = walk.template next<C::kNDV>(a, list, s);
+        float cq = 0.0f;
+        if (have) {
+            q_begin(s);
+            q_share(s);
+            if constexpr (C::kF32) soft_bar();
+            cq = q_finish(s);
+        }
+        while (have) {
+            const int n = s.j1 - s.j0;
+            const bool active = quarter * 32 < s.rows;    // a row of this warp belongs to the unit
+            const bool mine = row < s.rows;
             // ---- this warpgroup's tiles ----------------------------------------------------------
             float mref = 0.0f, l = 0.0f;
             bool any = false, had = false;
@@ -689,16 +796,16 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             for (int i = 0; i < n; ++i) {
                 const uint32_t t = tile + i, buf = t & 1u;
                 const uint32_t stream = C::kNS == 2 ? buf : 0;
-                const uint32_t sk = st + 2 * i, sv = sk + 1;
-                const bool my_tile = C::kNS == 1 || (int)buf == wg;
-                if (my_tile) {
+                const uint32_t sv = st + 2 * i + 1;             // the stage of the tile's values
+                if (C::kNS == 1 || (int)buf == wg) {
                     // This stream's last product complete.  With two streams S(t)
                     // complete already means it (it was issued first); with one
                     // stream every product is waited for, so that the barrier
                     // is never two phases ahead of a wait.
-                    bool waited = C::kNS == 2 || pv[stream] == 0;
+                    bool waited = C::kNS == 2 || pv0 == 0;
                     auto wait_pv = [&]() {
-                        if (!waited) ok = ok && warp_wait_fast(&ofull[stream], (pv[stream] - 1) & 1u, a.status);
+                        if (waited) return;
+                        ok = ok && warp_wait_fast(&ofull[0], (pv0 - 1) & 1u, a.status);
                         waited = true;
                         tc_after();
                     };
@@ -713,12 +820,12 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                             ok = ok && warp_wait_fast(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
                             uint8_t *v = smem + (sv % C::kStages) * C::kStage;
                             constexpr int kU = C::kSubW * 2 / 16;
-                            const int units = (kTile - valid) * kU * (HD / C::kSubW);
-                            for (int u = quarter * 32 + lane; u < units; u += 128) {
-                                const int c = u / ((kTile - valid) * kU), r = u % ((kTile - valid) * kU);
-                                *reinterpret_cast<uint4 *>(v + c * C::kSub + valid * C::kSubW * 2 + r * 16) =
-                                    make_uint4(0, 0, 0, 0);
-                            }
+                            const int units = (kTile - valid) * kU;
+#pragma unroll
+                            for (int c = 0; c < HD / C::kSubW; ++c)
+                                for (int u = quarter * 32 + lane; u < units; u += 128)
+                                    *reinterpret_cast<uint4 *>(v + c * C::kSub + valid * C::kSubW * 2 + u * 16) =
+                                        make_uint4(0, 0, 0, 0);
                             fence_async();
                         }
                     } else {
@@ -726,39 +833,59 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     }
                     if (active && ok) {
                         const uint32_t sc = lanes + kColS + buf * kTile;
-                        float x[kTile];
-                        tmem_ld32_nowait(sc, x);
-                        tmem_ld32_nowait(sc + 32, x + 32);
-                        tmem_wait_ld();
-                        if (valid < kTile) {
-#pragma unroll
-                            for (int j = 0; j < kTile; ++j)
-                                if (j >= valid) x[j] = -INFINITY;
-                        }
-                        float top = -INFINITY;
                         const float *sd = side + (t % kSide) * 16;
                         // never 0: -inf (a row past the end) times it has to stay -inf
                         auto factor = [&](int g) { return fmaxf(sd[g] * cq, 1e-37f); };
+                        // 16 bits: the tile's 64 scores stay in registers; F32, with fewer of
+                        // them, reads each half again for its weights
+                        constexpr int kHeld = C::kF32 ? 32 : 64;
+                        float x[kHeld];
+                        auto past_end = [&](float *y, int j0, int nj) {
+                            if (valid < kTile) {
+#pragma unroll
+                                for (int j = 0; j < nj; ++j)
+                                    if (j0 + j >= valid) y[j] = -INFINITY;
+                            }
+                        };
+                        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                         if constexpr (C::kF32) {
 #pragma unroll
-                            for (int g = 0; g < 8; ++g) {
-                                const float f = factor(g), e = sd[8 + g];
+                            for (int h = 1; h >= 0; --h) {
+                                tmem_ld32_nowait(sc + 32 * h, x);
+                                tmem_wait_ld();
+                                past_end(x, 32 * h, 32);
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) top = fmaxf(top, fmaf(x[8 * g + j], f, e));
+                                for (int g = 0; g < 4; ++g) {
+                                    const float f = factor(4 * h + g), e = sd[8 + 4 * h + g];
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j)
+                                        top4[j & 3] = fmaxf(top4[j & 3], fmaf(x[8 * g + j], f, e));
+                                }
+                                if (score) {
+                                    float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile + 32 * h);
+#pragma unroll
+                                    for (int j = 0; j < 32; j += 4) {
+                                        const float f = factor(4 * h + (j >> 3));
+                                        o[j >> 2] = make_float4(x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f);
+                                    }
+                                }
                             }
                         } else {
+                            tmem_ld32_nowait(sc, x);
+                            tmem_ld32_nowait(sc + 32, x + 32);
+                            tmem_wait_ld();
+                            past_end(x, 0, 64);
 #pragma unroll
-                            for (int j = 0; j < kTile; ++j) top = fmaxf(top, x[j]);
-                            top *= cq;
-                        }
-                        if (score) {
-                            float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile);
+                            for (int j = 0; j < kTile; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
+                            if (score) {
+                                float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile);
 #pragma unroll
-                            for (int j = 0; j < kTile; j += 4) {
-                                const float f = C::kF32 ? factor(j >> 3) : cq;
-                                o[j >> 2] = make_float4(x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f);
+                                for (int j = 0; j < kTile; j += 4)
+                                    o[j >> 2] = make_float4(x[j] * cq, x[j + 1] * cq, x[j + 2] * cq, x[j + 3] * cq);
                             }
                         }
+                        float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                        if constexpr (!C::kF32) top *= cq;
                         // ---- the reference exponent ----------------------------------------------------
                         const float want = top == -INFINITY ? (any ? mref : 0.0f) : rintf(top) - kShift;
                         if (!any) {
@@ -770,42 +897,41 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                             mref = to;
                             l *= f;
                             const uint32_t oc = lanes + C::kColO + stream * C::kDV;
+#pragma unroll 1
+                            for (int c = 0; c < C::kDV; c += 16) {
+                                float o[16];
+                                tmem_ld16(oc + c, o);
 #pragma unroll
-                            for (int c = 0; c < C::kDV; c += 32) {
-                                float o[32];
-                                tmem_ld32_nowait(oc + c, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] *= f;
-                                tmem_st32(oc + c, *reinterpret_cast<const uint32_t(*)[32]>(o));
+                                for (int j = 0; j < 16; ++j) o[j] *= f;
+                                tmem_st16(oc + c, reinterpret_cast<const uint32_t *>(o));
                             }
                         }
                         // ---- weights -------------------------------------------------------------------
-                        if constexpr (C::kF32) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                uint32_t w[32];
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t w[32];
+                            if constexpr (C::kF32) {
+                                if (h == 1) {       // the first half is still there
+                                    tmem_ld32_nowait(sc + 32, x);
+                                    tmem_wait_ld();
+                                    past_end(x, 32, 32);
+                                }
 #pragma unroll
-                                for (int g = 4 * h; g < 4 * h + 4; ++g) {
-                                    const float f = factor(g), e = sd[8 + g] - mref;
+                                for (int g = 0; g < 4; ++g) {
+                                    const float ev = sd[8 + 4 * h + g], f = factor(4 * h + g), e = ev - mref;
                                     float sum = 0.0f;
 #pragma unroll
                                     for (int j = 0; j < 8; j += 2) {
                                         const float p0 = ex2(fmaf(x[8 * g + j], f, e));
                                         const float p1 = ex2(fmaf(x[8 * g + j + 1], f, e));
                                         sum += p0 + p1;
-                                        const int o = 4 * (g - 4 * h) + (j >> 1);
+                                        const int o = 4 * g + (j >> 1);
                                         w[o] = split2<__half>(p0, p1, w[16 + o]);
                                     }
-                                    l = fmaf(sum, pow2(-(int)sd[8 + g]), l);
+                                    l = fmaf(sum, pow2(-(int)ev), l);
                                 }
-                                tmem_st32(sc + 32 * h, w);
-                            }
-                        } else {
-                            float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                uint32_t w[32];
+                            } else {
+                                float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
                                 for (int j = 0; j < 32; j += 2) {
                                     const float p0 = ex2(fmaf(x[32 * h + j], cq, -mref));
@@ -814,9 +940,9 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                                     l1 += p1;
                                     w[j >> 1] = split2<T>(p0, p1, w[16 + (j >> 1)]);
                                 }
-                                tmem_st32(sc + 32 * h, w);
+                                l += l0 + l1;
                             }
-                            l += l0 + l1;
+                            tmem_st32(sc + 32 * h, w);
                         }
                         tmem_wait_st();
                         any = true;
@@ -826,20 +952,31 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&pready[buf]);
                 }
-                ++pv[stream];
+                if (stream)
+                    ++pv1;
+                else
+                    ++pv0;
             }
 
-            // ---- the segment's partial: both streams' sums --------------------------------------------
-            // each warpgroup waits for its own stream's last product
-            {
+            // ---- the segment's end -----------------------------------------------------------------
+            // The next segment's Q is on its way while the last products run.  Each
+            // warpgroup waits for its own stream's last one; past the barrier every
+            // product is complete, Q and the score buffers are free, and the next
+            // scores can start while O is read.
+            const bool nhave = walk.template next<C::kNDV>(a, list, nx);
+            if (nhave) q_begin(nx);
+            if (had) {
                 const uint32_t k = C::kNS == 2 ? wg : 0;
-                if (had) ok = ok && warp_wait_fast(&ofull[k], (pv[k] - 1) & 1u, a.status);
+                ok = ok && warp_wait_fast(&ofull[k], ((k ? pv1 : pv0) - 1) & 1u, a.status);
             }
-            tc_before();
             ml[wg * kM + row] = make_float2(mref, l);
+            if (nhave) q_share(nx);
+            tc_before();
             soft_bar();
             tc_after();
-            float2 r0 = ml[row], r1 = C::kNS == 2 ? ml[kM + row] : make_float2(0.0f, 0.0f);
+            const float2 r0 = ml[row], r1 = C::kNS == 2 ? ml[kM + row] : make_float2(0.0f, 0.0f);
+            float cn = 0.0f;
+            if (nhave) cn = q_finish(nx);
             // a stream without a tile in this segment has nothing (the other has)
             const bool has0 = C::kNS == 1 || n > 1 || (tile & 1u) == 0, has1 = C::kNS == 2 && (n > 1 || (tile & 1u) == 1);
             const float m = has0 && has1 ? fmaxf(r0.x, r1.x) : has0 ? r0.x : r1.x;
@@ -852,48 +989,42 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 const int live = min(32, s.rows - quarter * 32);
                 if (wg == 0 && mine)
                     pm[lane] = make_float2(m, (has0 ? r0.y * f0 : 0.0f) + (has1 ? r1.y * f1 : 0.0f));
-                constexpr int kHalf = C::kDV / C::kNS, kP = kHalf < 32 ? kHalf : 32;
-                constexpr int kLpr = kP / 4, kRpi = 32 / kLpr;
-                const int lr = lane / kLpr, lu = lane % kLpr;
+                constexpr int kHalf = C::kDV / C::kNS, kP = 16;
+                constexpr int kOl = kP / 4, kOr = 32 / kOl;      // lanes of a row's piece, rows per store
+                const int olr = lane / kOl, olu = lane % kOl;
 #pragma unroll 1
                 for (int c = wg * kHalf; c < (wg + 1) * kHalf; c += kP) {
-                    float o[kP];
+                    float o[kP], v[kP];
+                    tmem_ld16_nowait(lanes + C::kColO + c, o);
+                    if constexpr (C::kNS == 2) tmem_ld16_nowait(lanes + C::kColO + C::kDV + c, v);
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < kP; ++k) o[k] = 0.0f;
-                    if (has0) {
-                        float v[16];
-#pragma unroll
-                        for (int k = 0; k < kP; k += 16) {
-                            tmem_ld16(lanes + C::kColO + c + k, v);
-#pragma unroll
-                            for (int q = 0; q < 16; ++q) o[k + q] = v[q] * f0;
-                        }
-                    }
-                    if (has1) {
-                        float v[16];
-#pragma unroll
-                        for (int k = 0; k < kP; k += 16) {
-                            tmem_ld16(lanes + C::kColO + C::kDV + c + k, v);
-#pragma unroll
-                            for (int q = 0; q < 16; ++q) o[k + q] = fmaf(v[q], f1, o[k + q]);
-                        }
+                    for (int k = 0; k < kP; ++k) {
+                        o[k] = has0 ? o[k] * f0 : 0.0f;
+                        if (C::kNS == 2 && has1) o[k] = fmaf(v[k], f1, o[k]);
                     }
 #pragma unroll
-                    for (int u = 0; u < kLpr; ++u)
+                    for (int u = 0; u < kOl; ++u)
                         *reinterpret_cast<float4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4)) =
                             make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
                     __syncwarp();
-                    for (int r = 0; r < live; r += kRpi)
-                        if (r + lr < live)
-                            *reinterpret_cast<float4 *>(po + (size_t)(r + lr) * C::kDV + c + 4 * lu) =
-                                *reinterpret_cast<const float4 *>(scratch + (r + lr) * 128 + ((lu ^ ((r + lr) & 7)) << 4));
+#pragma unroll
+                    for (int r = 0; r < 32; r += kOr)
+                        if (r + olr < live)
+                            *reinterpret_cast<float4 *>(po + (size_t)(r + olr) * C::kDV + c + 4 * olu) =
+                                *reinterpret_cast<const float4 *>(scratch + (r + olr) * 128 +
+                                                                  ((olu ^ ((r + olr) & 7)) << 4));
                     __syncwarp();
                 }
             }
             tc_before();
-            soft_bar();      // ml is free, and no warp writes Q while another reads O
+            __syncwarp();
+            if (lane == 0) mbar_arrive(oready);
             tile += n;
             st += 2 * n;
+            s = nx;
+            have = nhave;
+            cq = cn;
         }
     }
     __syncwarp();
@@ -921,7 +1052,7 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
     pdl_wait();
     pdl_launch_dependents();
     const int cum = __ldcg(a.cum + b), nt = __ldcg(a.cum + b + 1) - cum;
-    const List l(a, __ldcg(a.cum + a.n_seq));
+    const List l(a, C::kNDV, __ldcg(a.cum + a.n_seq));
     const int n_out = blockIdx.z == 0 ? C::kNDV : 1;    // the weights need one half's sums only
     const bool out = blockIdx.z == 0;
     for (int i = warp; i < a.group * n_out; i += kCombWarps) {
@@ -1025,8 +1156,6 @@ int ab_shape(const lalb_kv_batch *c, const lalb_attn_batch *p) {
     return LALB_OK;
 }
 
-constexpr int kGrid = 148;      // one CTA per SM of a B200 (workspace sizes need no device)
-
 struct Plan {
     AbArgs a;
     size_t o_cum, o_mlp, o_mlo, o_pp, o_po, o_score, bytes;
@@ -1043,17 +1172,16 @@ void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
     a.max_ctx = c->max_ctx;
     a.prefix = p->prefix_len;
     a.add_weights = p->add_weights != 0;
-    a.ndv = c->dtype == LALB_DT_F32 && c->head_dim == 256 ? 2 : 1;
+    const int ndv = c->dtype == LALB_DT_F32 && c->head_dim == 256 ? 2 : 1;   // Cfg::kNDV
     a.m_p = (a.n_seq * a.group + kM - 1) / kM;
     a.m_o = (a.group + kM - 1) / kM;
     a.rows_p = std::min(kM, a.n_seq * a.group);
     a.rows_o = std::min(kM, a.group);
-    a.grid = kGrid;
     a.pitch = tiles_of(a.max_ctx) * kTile;
-    const int dv = a.hd / a.ndv;
+    const int dv = a.hd / ndv;
     // a segment's slot is its CTA's number plus its unit's
-    const size_t sp = a.prefix ? (size_t)kGrid + (size_t)a.n_kv * a.m_p * a.ndv : 0;
-    const size_t so = (size_t)kGrid + (size_t)a.n_seq * a.n_kv * a.m_o * a.ndv;
+    const size_t sp = a.prefix ? (size_t)kGrid + (size_t)a.n_kv * a.m_p * ndv : 0;
+    const size_t so = (size_t)kGrid + (size_t)a.n_seq * a.n_kv * a.m_o * ndv;
     size_t off = 0;
     auto take = [&](size_t n) {
         const size_t at = off;
@@ -1168,7 +1296,7 @@ extern "C" int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache, c
             if (int st = map2d(ctx, &maps[i], base[i], dt, 2, (long long)a.n_kv * a.hd, rows, box, kTile, sw)) return st;
         }
     }
-    if (int st = launch_pdl(ctx, kn.tiles, dim3(a.grid), dim3(kn.threads), kn.smem, (cudaStream_t)stream,
+    if (int st = launch_pdl(ctx, kn.tiles, dim3(kGrid), dim3(kn.threads), kn.smem, (cudaStream_t)stream,
                             {&maps[0], &maps[1], &maps[2], &maps[3], &a}))
         return st;
     LALB_LAUNCH_CHECK(ctx, "attention_tiles_kernel");
