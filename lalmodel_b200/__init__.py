@@ -42,24 +42,25 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _want(who, name, t, device, dtype, numel=None, optional=False):
-    """Checks of a tensor whose address goes to the library."""
-    if t is None and optional:
-        return
-    ok = (isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype and t.is_contiguous()
-          and (numel is None or t.numel() == numel))
-    if not ok:
-        raise LalbError(who, -1, "%s must be a contiguous %s tensor%s on %s" %
-                        (name, dtype, "" if numel is None else " of %d elements" % numel, device))
+def _want(who, name, t, index, dtype, numel=None):
+    """Checks of a tensor whose address goes to the library (index: its CUDA
+    device); returns the address."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+            and (numel is None or t.numel() == numel)):
+        raise LalbError(who, -1, "%s must be a contiguous %s tensor%s on cuda:%d" %
+                        (name, dtype, "" if numel is None else " of %d elements" % numel, index))
+    return t.data_ptr()
 
 
-def _want_rows(who, name, t, device, dtype, rows, cols):
-    """Checks of a matrix whose rows may lie apart; returns their distance."""
-    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype and t.dim() == 2
-            and tuple(t.shape) == (rows, cols) and t.stride(1) == 1 and (rows < 2 or t.stride(0) >= cols)):
-        raise LalbError(who, -1, "%s must be a %s matrix [%d][%d] with contiguous rows on %s" %
-                        (name, dtype, rows, cols, device))
-    return t.stride(0) if rows > 1 else cols
+def _want_rows(who, name, t, index, dtype, rows, cols):
+    """Checks of a matrix whose rows may lie apart; returns its address and
+    their distance."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.shape == (rows, cols):
+        s0, s1 = t.stride()
+        if s1 == 1 and (rows < 2 or s0 >= cols):
+            return t.data_ptr(), s0 if rows > 1 else cols
+    raise LalbError(who, -1, "%s must be a %s matrix [%d][%d] with contiguous rows on cuda:%d" %
+                    (name, dtype, rows, cols, index))
 
 
 def unpack_scales_6bit(scales12):
@@ -166,8 +167,20 @@ class Context:
         return out
 
     # ---- a batch of sequences -----------------------------------------------
-    def _batch_stream(self):
-        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+    def _on(self, who, cache):
+        """The checks every call on a KVBatch makes: the device index."""
+        index = self.device.index
+        if cache.index != index:
+            raise LalbError(who, -1, "the cache is not on %s" % self.device)
+        return index
+
+    def _workspace(self, who, ws, index, need):
+        if ws is None:
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        p = _want(who, "ws", ws, index, torch.uint8)
+        if ws.numel() < need:
+            raise LalbError(who, -1, "ws holds %d bytes of %d" % (ws.numel(), need))
+        return ws, p
 
     def rope_append(self, cache, qkv, positions, slots, n_head, rope=None, out=None):
         """T tokens enter a KVBatch (lalb_rope_append): qkv [T][(n_head + 2
@@ -177,36 +190,30 @@ class Context:
         and the v to their rows and returns the rotated q [T][n_head *
         head_dim] in the cache's type."""
         who = "lalb_rope_append"
-        T = qkv.shape[0]
-        hd, width = cache.head_dim, n_head * cache.head_dim
-        cols = width + (0 if slots is None else 2 * cache.n_kv_head * hd)
-        cache.check(who, self.device)
-        if qkv.dtype not in (torch.float32, cache.k.dtype):
+        index, dt = self._on(who, cache), cache.dtype
+        T, width = qkv.shape[0], n_head * cache.head_dim
+        if qkv.dtype is not torch.float32 and qkv.dtype is not dt:
             raise LalbError(who, -1, "qkv must be float32 or of the cache's type")
-        stride = _want_rows(who, "qkv", qkv, self.device, qkv.dtype, T, cols)
-        _want(who, "positions", positions, self.device, torch.int32, T)
-        _want(who, "slots", slots, self.device, torch.int32, T, optional=True)
+        p, stride = _want_rows(who, "qkv", qkv, index, qkv.dtype, T, width + (0 if slots is None else 2 * cache.kvr))
+        pos = _want(who, "positions", positions, index, torch.int32, T)
+        sl = None if slots is None else _want(who, "slots", slots, index, torch.int32, T)
         if out is None:
-            out = torch.empty((T, width), dtype=cache.k.dtype, device=self.device)
-        _want(who, "out", out, self.device, cache.k.dtype, T * width)
+            out = torch.empty((T, width), dtype=dt, device=self.device)
+        o = _want(who, "out", out, index, dt, T * width)
         if T == 0:
             return out
-        self._call(who, self.h, ctypes.byref((rope or Rope()).desc), ctypes.byref(cache.desc), n_head, _p(qkv),
-                   _DT[qkv.dtype], stride, T, _p(positions), _p(slots), _p(out), self._batch_stream())
-        return out
+        st = _abi.lib().lalb_rope_append(self.h, (rope or _DEFAULT_ROPE).ref, cache.ref, n_head, p, _DT[qkv.dtype],
+                                         stride, T, pos, sl, o, torch._C._cuda_getCurrentRawStream(index))
+        return out if st == 0 else self._raise(who, st)
+
+    def _raise(self, who, st):
+        raise LalbError(who, st, _abi.lib().lalb_last_error(self.h).decode())
 
     def attention_batch_ws(self, cache, n_head, prefix_len=0, weights=False):
         """Workspace of attention_batch calls with a prefix of prefix_len rows
         at most."""
-        a = _abi.AttnBatchDesc(n_head, 0.0, prefix_len, None, None, int(weights), 0.0)
-        return self._batch_ws("lalb_attention_batch_ws_bytes", ctypes.byref(cache.desc), ctypes.byref(a))
-
-    def _batch_ws(self, name, *args):
-        n = ctypes.c_size_t()
-        st = getattr(_abi.lib(), name)(*args, ctypes.byref(n))
-        if st:
-            raise LalbError(name, st)
-        return torch.empty(n.value, dtype=torch.uint8, device=self.device)
+        return torch.empty(cache.attention_bytes(n_head, prefix_len, bool(weights)), dtype=torch.uint8,
+                           device=self.device)
 
     def attention_batch(self, cache, q, lens, n_head, prefix_k=None, prefix_v=None, scale=0.0, decay=None,
                         ws=None, out=None):
@@ -217,38 +224,28 @@ class Context:
         cache's row_weight = decay * row_weight + this step's weights.
         Returns out [n_seq][n_head * head_dim]."""
         who = "lalb_attention_batch"
-        cache.check(who, self.device)
-        width, kvr, dt = n_head * cache.head_dim, cache.n_kv_head * cache.head_dim, cache.k.dtype
-        stride = _want_rows(who, "q", q, self.device, dt, cache.n_seq, width)
-        _want(who, "lens", lens, self.device, torch.int32, cache.n_seq)
-        prefix = 0
-        if (prefix_k is None) != (prefix_v is None):
-            raise LalbError(who, -1, "prefix_k and prefix_v come together")
-        if prefix_k is not None:
-            prefix = prefix_k.numel() // kvr
-            _want(who, "prefix_k", prefix_k, self.device, dt, prefix * kvr)
-            _want(who, "prefix_v", prefix_v, self.device, dt, prefix * kvr)
-        a = _abi.AttnBatchDesc(n_head, scale, prefix, _p(prefix_k) if prefix else None,
-                               _p(prefix_v) if prefix else None, int(decay is not None), decay or 0.0)
-        n = ctypes.c_size_t()
-        st = _abi.lib().lalb_attention_batch_ws_bytes(ctypes.byref(cache.desc), ctypes.byref(a), ctypes.byref(n))
-        if st:
-            raise LalbError("lalb_attention_batch_ws_bytes", st)
-        if ws is None:
-            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
-        _want(who, "ws", ws, self.device, torch.uint8)
-        if ws.numel() < n.value:
-            raise LalbError(who, -1, "ws holds %d bytes of %d" % (ws.numel(), n.value))
+        index, dt, width = self._on(who, cache), cache.dtype, n_head * cache.head_dim
+        p, stride = _want_rows(who, "q", q, index, dt, cache.n_seq, width)
+        n = _want(who, "lens", lens, index, torch.int32, cache.n_seq)
+        prefix, pk, pv = 0, None, None
+        if prefix_k is not None or prefix_v is not None:
+            if prefix_k is None or prefix_v is None:
+                raise LalbError(who, -1, "prefix_k and prefix_v come together")
+            prefix = prefix_k.numel() // cache.kvr
+            pk = _want(who, "prefix_k", prefix_k, index, dt, prefix * cache.kvr)
+            pv = _want(who, "prefix_v", prefix_v, index, dt, prefix * cache.kvr)
+        a = _abi.AttnBatchDesc(n_head, scale, prefix, pk, pv, decay is not None, decay or 0.0)
+        ws, w = self._workspace(who, ws, index, cache.attention_bytes(n_head, prefix, decay is not None))
         if out is None:
             out = torch.empty((cache.n_seq, width), dtype=dt, device=self.device)
-        _want(who, "out", out, self.device, dt, cache.n_seq * width)
-        self._call(who, self.h, ctypes.byref(cache.desc), ctypes.byref(a), _p(q), stride, _p(lens), _p(ws), _p(out),
-                   self._batch_stream())
-        return out
+        o = _want(who, "out", out, index, dt, cache.n_seq * width)
+        st = _abi.lib().lalb_attention_batch(self.h, cache.ref, ctypes.byref(a), p, stride, n, w, o,
+                                             torch._C._cuda_getCurrentRawStream(index))
+        return out if st == 0 else self._raise(who, st)
 
     def kv_evict_ws(self, cache, keep):
         """Workspace of kv_evict calls that keep `keep` rows."""
-        return self._batch_ws("lalb_kv_evict_ws_bytes", ctypes.byref(cache.desc), keep)
+        return torch.empty(cache.evict_bytes(keep), dtype=torch.uint8, device=self.device)
 
     def kv_evict(self, cache, lens, keep, n_sink=0, n_recent=0, ws=None):
         """Cuts every sequence of a KVBatch to the `keep` rows that matter
@@ -256,19 +253,13 @@ class Context:
         the largest row_weight.  Updates the cache, its row_pos and row_weight
         and lens (int32 [n_seq])."""
         who = "lalb_kv_evict"
-        cache.check(who, self.device)
-        _want(who, "lens", lens, self.device, torch.int32, cache.n_seq)
-        n = ctypes.c_size_t()
-        st = _abi.lib().lalb_kv_evict_ws_bytes(ctypes.byref(cache.desc), keep, ctypes.byref(n))
+        index = self._on(who, cache)
+        n = _want(who, "lens", lens, index, torch.int32, cache.n_seq)
+        ws, w = self._workspace(who, ws, index, cache.evict_bytes(keep))
+        st = _abi.lib().lalb_kv_evict(self.h, cache.ref, n, keep, n_sink, n_recent, w,
+                                      torch._C._cuda_getCurrentRawStream(index))
         if st:
-            raise LalbError("lalb_kv_evict_ws_bytes", st, "keep %d" % keep)
-        if ws is None:
-            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
-        _want(who, "ws", ws, self.device, torch.uint8)
-        if ws.numel() < n.value:
-            raise LalbError(who, -1, "ws holds %d bytes of %d" % (ws.numel(), n.value))
-        self._call(who, self.h, ctypes.byref(cache.desc), _p(lens), keep, n_sink, n_recent, _p(ws),
-                   self._batch_stream())
+            self._raise(who, st)
 
     def sample(self, logits, history=None, temperature=0.0, top_k=1, top_p=0.9,
                rep_penalty=1.0, no_repeat_ngram=0, n_masked_low_ids=0, u=None, want_topk=False):
@@ -330,25 +321,49 @@ class KVBatch:
     """One layer's KV cache for a batch of sequences (include/lalb.h,
     lalb_kv_batch): k, v CUDA tensors [n_seq][max_ctx][n_kv_head * head_dim]
     (float32, float16 or bfloat16); row_pos int32 and row_weight float32
-    [n_seq][n_kv_head][max_ctx], both optional."""
+    [n_seq][n_kv_head][max_ctx], both optional.  The tensors are checked here,
+    once, and stay the cache's."""
 
     def __init__(self, k, v, n_kv_head, row_pos=None, row_weight=None):
         if k.dim() != 3 or k.dtype not in _DT or n_kv_head < 1 or k.shape[2] % n_kv_head:
             raise LalbError("KVBatch", -1, "k must be a float32, float16 or bfloat16 tensor "
                                            "[n_seq][max_ctx][n_kv_head * head_dim]")
         self.k, self.v, self.row_pos, self.row_weight = k, v, row_pos, row_weight
-        self.n_seq, self.max_ctx = k.shape[0], k.shape[1]
+        self.n_seq, self.max_ctx, self.kvr = k.shape
         self.n_kv_head, self.head_dim = n_kv_head, k.shape[2] // n_kv_head
-        self.check("KVBatch", k.device)
-        self.desc = _abi.KVBatchDesc(_DT[k.dtype], self.n_seq, self.max_ctx, n_kv_head, self.head_dim, _p(k), _p(v),
-                                     _p(row_pos), _p(row_weight))
+        self.dtype, self.index = k.dtype, k.get_device()
+        rows = self.n_seq * n_kv_head * self.max_ctx
+        self.desc = _abi.KVBatchDesc(
+            _DT[k.dtype], self.n_seq, self.max_ctx, n_kv_head, self.head_dim,
+            _want("KVBatch", "k", k, self.index, k.dtype), _want("KVBatch", "v", v, self.index, k.dtype, k.numel()),
+            None if row_pos is None else _want("KVBatch", "row_pos", row_pos, self.index, torch.int32, rows),
+            None if row_weight is None else _want("KVBatch", "row_weight", row_weight, self.index, torch.float32,
+                                                  rows))
+        self.ref = ctypes.byref(self.desc)
+        self._bytes = {}
 
-    def check(self, who, device):
-        rows = self.n_seq * self.n_kv_head * self.max_ctx
-        _want(who, "k", self.k, device, self.k.dtype)
-        _want(who, "v", self.v, device, self.k.dtype, self.k.numel())
-        _want(who, "row_pos", self.row_pos, device, torch.int32, rows, optional=True)
-        _want(who, "row_weight", self.row_weight, device, torch.float32, rows, optional=True)
+    def _ws_bytes(self, name, key, *args):
+        n = self._bytes.get(key)
+        if n is None:
+            out = ctypes.c_size_t()
+            st = getattr(_abi.lib(), name)(self.ref, *args, ctypes.byref(out))
+            if st:
+                raise LalbError(name, st, str(key))
+            n = self._bytes[key] = out.value
+        return n
+
+    def attention_bytes(self, n_head, prefix_len, weights):
+        """Workspace bytes of lalb_attention_batch on this cache."""
+        key = (n_head, prefix_len, weights)
+        n = self._bytes.get(key)
+        if n is None:
+            a = _abi.AttnBatchDesc(n_head, 0.0, prefix_len, None, None, weights, 0.0)
+            n = self._ws_bytes("lalb_attention_batch_ws_bytes", key, ctypes.byref(a))
+        return n
+
+    def evict_bytes(self, keep):
+        """Workspace bytes of lalb_kv_evict on this cache."""
+        return self._ws_bytes("lalb_kv_evict_ws_bytes", keep, keep)
 
 
 class Rope:
@@ -365,6 +380,10 @@ class Rope:
             raise LalbError("Rope", -1, "layout %r, scaling %r" % (layout, scaling))
         self.desc = _abi.RopeDesc(self.LAYOUTS[layout], rot_dim, theta, self.SCALINGS[scaling], factor, orig_ctx,
                                   turns_fast, turns_slow, mscale)
+        self.ref = ctypes.byref(self.desc)
+
+
+_DEFAULT_ROPE = Rope()
 
 
 def prefill_ws_bytes(rows, K, T):

@@ -250,6 +250,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
         : "memory");
 }
 
+// The value every lane holds anyway, known to the compiler as one for the
+// warp: the MMA operands derived from it are computed in uniform registers
+// instead of moved there one by one for each instruction.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // A warpgroup's registers from here on (0: as launched).  In the role's own
 // branch: where roles meet again the compiler keeps to the smaller share.
 template <int N, bool INC>
@@ -582,7 +587,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 return false;
             tc_after();
             const uint32_t stream = C::kNS == 2 ? buf : 0;
-            const uint32_t d = C::kColO + stream * C::kDV, p = kColS + buf * kTile, v = ring + sv * C::kStage;
+            const uint32_t d = uniform(C::kColO + stream * C::kDV), p = uniform(kColS + buf * kTile);
+            const uint32_t v = uniform(ring + sv * C::kStage);
             // weights: high parts at 32 h + 0..15 of the buffer, the rest 16 columns on
             auto hi = [&](int kk) { return p + 32 * (kk >> 1) + 8 * (kk & 1); };
             auto v_off = [&](int kk) { return v + kk * 16 * C::kSubW * 2; };
@@ -611,7 +617,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     const uint32_t sk = st % C::kStages, use = st / C::kStages;
                     if (!(ok = warp_wait_fast(&full[sk], use & 1u, a.status))) break;
                     tc_after();
-                    const uint32_t d = kColS + buf * kTile, k = ring + sk * C::kStage;
+                    const uint32_t d = uniform(kColS + buf * kTile), k = uniform(ring + sk * C::kStage);
                     auto k_off = [&](int kk) {
                         return k + (kk / (C::kSubW / 16)) * C::kSub + (kk % (C::kSubW / 16)) * 32;
                     };

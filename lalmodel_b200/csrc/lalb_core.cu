@@ -82,15 +82,21 @@ extern "C" int lalb_init(int device, lalb_ctx **out) {
         cudaGetLastError();
         return LALB_ERR_DEVICE;
     }
-    cudaDeviceProp prop;
-    if (cudaGetDeviceProperties(&prop, device) != cudaSuccess) return LALB_ERR_CUDA;
-    if (prop.major != 10 || prop.minor != 0) return LALB_ERR_DEVICE;
+    // the four attributes needed: cudaGetDeviceProperties collects all of them,
+    // some slow to read (1 ms a call)
+    int major = 0, minor = 0, sms = 0, optin = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, device) != cudaSuccess)
+        return LALB_ERR_CUDA;
+    if (major != 10 || minor != 0) return LALB_ERR_DEVICE;
     if (cudaSetDevice(device) != cudaSuccess) return LALB_ERR_CUDA;
     lalb_ctx *ctx = new (std::nothrow) lalb_ctx();
     if (!ctx) return LALB_ERR_NOMEM;
     ctx->device = device;
-    ctx->sm_count = prop.multiProcessorCount;
-    ctx->smem_optin = prop.sharedMemPerBlockOptin;
+    ctx->sm_count = sms;
+    ctx->smem_optin = (size_t)optin;
     if (cudaMalloc(&ctx->scratch, sizeof(lalb_scratch)) != cudaSuccess) {
         delete ctx;
         return LALB_ERR_NOMEM;
