@@ -61,7 +61,6 @@ constexpr int kM = 128;              // query rows per unit
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (loaders run at most 5 ahead)
 constexpr float kShift = 6.0f;       // weights up to 2^6 at the reference maximum, 2^14 before a rescale
 constexpr float kGrow = 8.0f;        // growth of a row's maximum that is left in place
-constexpr int kColS = 0, kColQ = 128;
 constexpr int kStageBudget2 = 160 * 1024, kStageBudget1 = 192 * 1024;
 
 template <class T, int HD>
@@ -72,9 +71,15 @@ struct Cfg {
     static constexpr int kDV = kF32 && HD == 256 ? 128 : HD;
     static constexpr int kNDV = HD / kDV;
     static constexpr int kQCols = kF32 ? HD : HD / 2;
-    static constexpr int kNS = kColQ + kQCols + 2 * kDV <= 512 ? 2 : 1;   // softmax streams
-    static constexpr int kColO = 512 - kNS * kDV;
-    static_assert(kColQ + kQCols <= kColO, "Q and O fit TMEM");
+    static constexpr int kNS = 2 * kTile + kQCols + 2 * kDV <= 512 ? 2 : 1;   // softmax streams
+    // score buffers: S runs kBufs - 1 tiles ahead of PV.  With two streams and
+    // one tile ahead a stream's next scores wait behind its own last product
+    // (2.1 us for a pair of tiles whose products take 0.8); a third buffer
+    // needs 64 columns that F32 at head_dim 128 does not have
+    static constexpr int kBufs = kNS == 2 && 3 * kTile + kQCols + 2 * kDV <= 512 ? 3 : 2;
+    static constexpr int kAhead = kBufs - 1;
+    static constexpr int kColS = 0, kColQ = kBufs * kTile, kColO = 512 - kNS * kDV;
+    static_assert(kColQ + kQCols <= kColO, "the buffers, Q and O fit TMEM");
     static constexpr int kSoftWarps = 4 * kNS;
     // F32: 7, which with the MMA warp makes two warpgroups
     static constexpr int kLoadWarps = kF32 ? 7 : 1;
@@ -84,21 +89,21 @@ struct Cfg {
     // Registers a thread: the launch's even share, and the split of it (the
     // softmax holds a tile's scores and weights; at the even share it spills)
     static constexpr int kEven = kThreads == 512 ? 128 : kThreads == 384 ? 168 : 248;
-    static constexpr int kSoftRegs = kF32 ? (kNS == 2 ? 152 : 232) : kNS == 2 ? 216 : 0;   // 0: no split
-    static constexpr int kOtherRegs = kF32 ? (kNS == 2 ? 104 : 136) : 72;
+    static constexpr int kSoftRegs = kF32 ? (kNS == 2 ? 152 : 232) : kNS == 2 ? 208 : 0;   // 0: no split
+    static constexpr int kOtherRegs = kF32 ? (kNS == 2 ? 104 : 136) : 88;
     static_assert(kSoftRegs == 0 || kSoftRegs * kSoftWarps + kOtherRegs * kOtherWarps <=
                                         kEven * (kSoftWarps + kOtherWarps),
                   "the split is no more than the block was launched with");
     static constexpr uint32_t kStage = kTile * HD * (kF32 ? 4 : 2);
     static constexpr int kBudget = kNS == 2 ? kStageBudget2 : kStageBudget1;
     static constexpr int kStages = kBudget / (int)kStage < 10 ? kBudget / (int)kStage : 10;
-    static_assert(kStages >= 3, "K(j), V(j) and K(j + 1) are held at once");
+    static_assert(kStages >= 2 * kAhead + 1, "V(j) to K(j + kAhead) are held at once");
     static_assert(kStages / 2 + 2 <= kSide, "a tile's scales outlive its stages");
     static constexpr int kSubW = HD < 64 ? HD : 64;                   // columns of a swizzled subtile
     static constexpr uint32_t kSub = kTile * kSubW * 2;               // its bytes
     static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
     static constexpr uint32_t kOffMl = kOffScratch + kSoftWarps * 4096;
-    static constexpr uint32_t kOffSide = kOffMl + 2 * kM * 8 + (kF32 ? 2 * kM * 4 : 0);   // ml, and F32's qmax
+    static constexpr uint32_t kOffSide = kOffMl + 2 * kM * 8 + (kF32 ? 32 : 0);   // ml, and F32's qmax
     static constexpr uint32_t kOffBar = kOffSide + kSide * 16 * 4;
     static constexpr uint32_t kSmem = 1024 + kOffBar + 512;
     static_assert(kSmem <= 232448, "fits the 227 KB opt-in shared memory");
@@ -185,6 +190,7 @@ struct Walk {
             s.b = 0;
         } else {
             const int o = t - l.tp;
+#pragma unroll 1
             while (o >= c0 + nt * l.units_o) {
                 c0 += nt * l.units_o;
                 ++b;
@@ -211,6 +217,23 @@ struct Walk {
 };
 
 // ---- small PTX helpers -----------------------------------------------------------
+// mbar_wait_bounded and warp_wait_fast with the retry loop kept rolled: the
+// compiler unrolls its constant count at each of some twenty places, 55 KB of
+// code in a kernel whose warps each run most of their path once or a few times
+// and then wait for instructions.
+__device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, unsigned int *status) {
+    if (mbar_test_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (uint32_t i = 0; i < LALB_SPIN_LIMIT; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    atomicOr(status, LALB_STATUS_WAIT_TIMEOUT);
+    return false;
+}
+// Every lane of the warp, which goes on only when all of them saw the phase complete.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, unsigned int *status) {
+    return __all_sync(0xffffffffu, wait_bounded(bar, parity, status));
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -383,9 +406,9 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     float *side = reinterpret_cast<float *>(smem + C::kOffSide);      // [tile % kSide][K 8, V 8]
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
     uint64_t *empty = full + C::kStages;
-    uint64_t *sfull = empty + C::kStages;      // S(j) complete (and every product before it)
-    uint64_t *pready = sfull + 2;              // P(j) written
-    uint64_t *ofull = pready + 2;              // a stream's latest PV complete
+    uint64_t *sfull = empty + C::kStages;      // S(j) complete (and every product issued before it)
+    uint64_t *pready = sfull + C::kBufs;       // P(j) written
+    uint64_t *ofull = pready + C::kBufs;       // a stream's latest PV complete
     uint64_t *qready = ofull + 2;              // Q of the segment written
     uint64_t *oready = qready + 1;             // O of the segment read
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(oready + 1);
@@ -398,11 +421,11 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             mbar_init(&full[s], C::kFullCount);
             mbar_init(&empty[s], 1);
         }
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < C::kBufs; ++s) {
             mbar_init(&sfull[s], 1);
             mbar_init(&pready[s], 4);
-            mbar_init(&ofull[s], 1);
         }
+        for (int s = 0; s < 2; ++s) mbar_init(&ofull[s], 1);
         mbar_init(qready, C::kSoftWarps);
         mbar_init(oready, C::kSoftWarps);
         fence_barrier_init();
@@ -416,12 +439,13 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     }
     pdl_wait();
     // ---- the list: its length, and where this CTA's own tiles begin ---------------------
+    // the lengths, one read for all of them (the softmax warps' scratch holds them)
+    int *lens_s = reinterpret_cast<int *>(smem + C::kOffScratch);
+    constexpr int kHeld = C::kSoftWarps * 4096 / 4;
+    for (int b = threadIdx.x; b < a.n_seq && b < kHeld; b += C::kThreads) lens_s[b] = __ldcg(a.lens + b);
+    __syncthreads();
     if (warp == 0) {
-        // tiles of 32 sequences at a time, the first kHold x 32 of them loaded
-        // together and kept for the second look
-        constexpr int kHold = 8;
-        int held[kHold];
-        auto length = [&](int b) { return b < a.n_seq ? __ldcg(a.lens + b) : 0; };
+        auto length = [&](int b) { return b >= a.n_seq ? 0 : b < kHeld ? lens_s[b] : __ldcg(a.lens + b); };
         auto tiles = [&](int n) { return n < 0 || n > a.max_ctx ? 0 : tiles_of(n); };
         auto scan = [&](int x) {
 #pragma unroll
@@ -431,46 +455,37 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             }
             return x;
         };
-#pragma unroll
-        for (int i = 0; i < kHold; ++i) held[i] = length(32 * i + lane);
         int sum = 0;
-        auto look = [&](int b0, int n) {
-            if (n < 0 || n > a.max_ctx) {
-                if (blockIdx.x == 0) atomicOr(a.status, LALB_STATUS_BAD_POSITION);
+#pragma unroll 1
+        for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+            const int n = length(b0 + lane), nt = tiles(n), incl = scan(nt);
+            if (blockIdx.x == 0) {
+                if (n < 0 || n > a.max_ctx) atomicOr(a.status, LALB_STATUS_BAD_POSITION);
+                if (b0 + lane < a.n_seq) a.cum[b0 + lane] = sum + incl - nt;
             }
-            const int incl = scan(tiles(n));
-            if (blockIdx.x == 0 && b0 + lane < a.n_seq) a.cum[b0 + lane] = sum + incl - tiles(n);
             sum += __shfl_sync(0xffffffffu, incl, 31);
-        };
-#pragma unroll
-        for (int i = 0; i < kHold; ++i)
-            if (32 * i < a.n_seq) look(32 * i, held[i]);
-        for (int b0 = 32 * kHold; b0 < a.n_seq; b0 += 32) look(b0, length(b0 + lane));
+        }
         if (blockIdx.x == 0 && lane == 0) a.cum[a.n_seq] = sum;
         const List l(a, C::kNDV, sum);
         const int first = l.first(blockIdx.x) - l.tp;   // among the own tiles
         // the sequence of that tile (the first one, if the CTA begins in the prefix)
         const int want = first > 0 ? first / l.units_o : 0;
-        int sb = 0, before = 0, n0 = __shfl_sync(0xffffffffu, held[0], 0);
+        int sb = 0, before = 0, n0 = length(0);
         if (first > 0 && first < sum * l.units_o) {     // cum[sb] <= want < cum[sb + 1]
             int run = 0;
-            bool found = false;
-            auto find = [&](int b0, int n) {
-                const int nt = tiles(n), incl = scan(nt);
+#pragma unroll 1
+            for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+                const int n = length(b0 + lane), nt = tiles(n), incl = scan(nt);
                 const uint32_t past = __ballot_sync(0xffffffffu, run + incl > want);
                 if (past) {
                     const int i = __ffs(past) - 1;
                     sb = b0 + i;
                     before = run + __shfl_sync(0xffffffffu, incl - nt, i);
                     n0 = __shfl_sync(0xffffffffu, n, i);
-                    found = true;
+                    break;
                 }
                 run += __shfl_sync(0xffffffffu, incl, 31);
-            };
-#pragma unroll
-            for (int i = 0; i < kHold; ++i)
-                if (!found && 32 * i < a.n_seq) find(32 * i, held[i]);
-            for (int b0 = 32 * kHold; !found && b0 < a.n_seq; b0 += 32) find(b0, length(b0 + lane));
+            }
         }
         if (lane == 0) {
             *start_b = sb;
@@ -516,7 +531,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             auto finish = [&](auto &x, int g, bool is_v) {
                 const int e = x.exponent();
                 const uint32_t slot = st % C::kStages, use = st / C::kStages;
-                if (use > 0) ok = ok && warp_wait_fast(&empty[slot], (use - 1) & 1u, a.status);
+                if (use > 0) ok = ok && warp_wait(&empty[slot], (use - 1) & 1u, a.status);
                 x.store(smem + slot * C::kStage, 8 * g, pow2(-e), lane);
                 // K: the factor that undoes the scaling; V: the exponent
                 if (lane == 0) side[(tile % kSide) * 16 + (is_v ? 8 : 0) + g] = is_v ? (float)e : pow2(e);
@@ -524,12 +539,15 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[slot]);
             };
+#pragma unroll 1
             while (walk.template next<C::kNDV>(a, list, s)) {
                 const size_t seq = s.prefix ? 0 : (size_t)s.b * a.max_ctx * pitch;
                 const float *kb = static_cast<const float *>(s.prefix ? a.pk : a.k) + seq + (size_t)s.g * HD;
                 const float *vb =
                     static_cast<const float *>(s.prefix ? a.pv : a.v) + seq + (size_t)s.g * HD + s.dv * C::kDV;
+#pragma unroll 1
                 for (int j = s.j0; j < s.j1 && ok; ++j, ++tile) {
+#pragma unroll 1
                     for (int g = turn; g < 8; g += C::kLoadWarps) {
                         RowLoad<HD> x;
                         group(x, kb, j, s.n, g);
@@ -537,6 +555,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     }
                     ++st;
                     turn = (turn + 6) % 7;          // 8 groups on: -8 = 6 mod 7
+#pragma unroll 1
                     for (int g = turn; g < 8; g += C::kLoadWarps) {
                         RowLoad<C::kDV> x;
                         group(x, vb, j, s.n, g);
@@ -549,13 +568,16 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         } else if (lane == 0) {
             uint32_t st = 0;
             bool ok = true;
+#pragma unroll 1
             while (walk.template next<C::kNDV>(a, list, s)) {
                 const CUtensorMap *mk = s.prefix ? &mPK : &mK, *mv = s.prefix ? &mPV : &mV;
                 const int row0 = s.prefix ? 0 : s.b * a.max_ctx;
+#pragma unroll 1
                 for (int j = s.j0; j < s.j1 && ok; ++j)
+#pragma unroll 1
                     for (int kv = 0; kv < 2 && ok; ++kv, ++st) {
                         const uint32_t slot = st % C::kStages, use = st / C::kStages;
-                        if (use > 0 && !mbar_wait_bounded(&empty[slot], (use - 1) & 1u, a.status)) {
+                        if (use > 0 && !wait_bounded(&empty[slot], (use - 1) & 1u, a.status)) {
                             ok = false;
                             break;
                         }
@@ -567,8 +589,9 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     }
             }
             // nothing may still be on its way into this CTA's shared memory when it ends
+#pragma unroll 1
             for (uint32_t i = st > (uint32_t)C::kStages ? st - C::kStages : 0; i < st; ++i)
-                mbar_wait_bounded(&full[i % C::kStages], (i / C::kStages) & 1u, a.status);
+                wait_bounded(&full[i % C::kStages], (i / C::kStages) & 1u, a.status);
         }
     } else if (warp == C::kSoftWarps) {
         // ================================ MMA ====================================================
@@ -577,26 +600,24 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         constexpr uint32_t kIdO = mma_idesc<typename std::conditional<C::kF32, __half, T>::type>(C::kDV, true);
         constexpr uint32_t kLoK = kTile * HD * 2, kLoV = kTile * C::kDV * 2;
         const uint32_t ring = smem_u32(smem);
-        uint32_t st = 0, tile = 0, segs = 0;
-        uint32_t vslot = 0;
+        uint32_t tile = 0, segs = 0;        // tiles before the segment: its K(i) is stage 2 (tile + i)
         bool ok = true;
-        auto issue_pv = [&](uint32_t t, uint32_t sv, uint32_t sv_use, bool first) -> bool {
-            const uint32_t buf = t & 1u;
-            if (!warp_wait_fast(&pready[buf], (t >> 1) & 1u, a.status) ||
-                !warp_wait_fast(&full[sv], sv_use & 1u, a.status))
+        auto issue_pv = [&](uint32_t t, bool first) -> bool {
+            const uint32_t buf = t % C::kBufs, sv = (2 * t + 1) % C::kStages, use = (2 * t + 1) / C::kStages;
+            if (!warp_wait(&pready[buf], (t / C::kBufs) & 1u, a.status) ||
+                !warp_wait(&full[sv], use & 1u, a.status))
                 return false;
             tc_after();
-            const uint32_t stream = C::kNS == 2 ? buf : 0;
-            const uint32_t d = uniform(C::kColO + stream * C::kDV), p = uniform(kColS + buf * kTile);
-            const uint32_t v = uniform(ring + sv * C::kStage);
-            // weights: high parts at 32 h + 0..15 of the buffer, the rest 16 columns on
-            auto hi = [&](int kk) { return p + 32 * (kk >> 1) + 8 * (kk & 1); };
+            const uint32_t stream = C::kNS == 2 ? t & 1u : 0;
+            const uint32_t d = C::kColO + stream * C::kDV, p = C::kColS + buf * kTile, v = ring + sv * C::kStage;
+            // weights: of 16 scores' 16 columns, 8 hold the high parts, 8 the rest
+            auto hi = [&](int kk) { return p + 16 * kk; };
             auto v_off = [&](int kk) { return v + kk * 16 * C::kSubW * 2; };
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; ++kk) {
                 if constexpr (C::kF32)
                     mma_f16_ta(d, hi(kk), mnmajor_desc<C::kSubW>(v_off(kk) + kLoV), kIdO, first && kk == 0 ? 0u : 1u);
-                mma_f16_ta(d, hi(kk) + 16, mnmajor_desc<C::kSubW>(v_off(kk)), kIdO,
+                mma_f16_ta(d, hi(kk) + 8, mnmajor_desc<C::kSubW>(v_off(kk)), kIdO,
                            first && kk == 0 && !C::kF32 ? 0u : 1u);
             }
 #pragma unroll
@@ -606,18 +627,20 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             commit_elect(&ofull[stream]);
             return true;
         };
+#pragma unroll 1
         while (ok && walk.template next<C::kNDV>(a, list, s)) {
-            if (!(ok = warp_wait_fast(qready, segs & 1u, a.status))) break;
+            if (!(ok = warp_wait(qready, segs & 1u, a.status))) break;
             tc_after();
             ++segs;
             const int n = s.j1 - s.j0;
-            for (int i = 0; i <= n; ++i) {
+#pragma unroll 1
+            for (int i = 0; i < n + C::kAhead && ok; ++i) {
                 if (i < n) {
-                    const uint32_t t = tile + i, buf = t & 1u;
-                    const uint32_t sk = st % C::kStages, use = st / C::kStages;
-                    if (!(ok = warp_wait_fast(&full[sk], use & 1u, a.status))) break;
+                    const uint32_t t = tile + i, buf = t % C::kBufs;
+                    const uint32_t sk = 2 * t % C::kStages, use = 2 * t / C::kStages;
+                    if (!(ok = warp_wait(&full[sk], use & 1u, a.status))) break;
                     tc_after();
-                    const uint32_t d = uniform(kColS + buf * kTile), k = uniform(ring + sk * C::kStage);
+                    const uint32_t d = C::kColS + buf * kTile, k = ring + sk * C::kStage;
                     auto k_off = [&](int kk) {
                         return k + (kk / (C::kSubW / 16)) * C::kSub + (kk % (C::kSubW / 16)) * 32;
                     };
@@ -627,26 +650,22 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     if constexpr (C::kF32) {
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
-                            mma_f16_ta(d, kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS, kk ? 1u : 0u);
-                            mma_f16_ta(d, kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, 1u);
+                            mma_f16_ta(d, C::kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS, kk ? 1u : 0u);
+                            mma_f16_ta(d, C::kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, 1u);
                         }
                     }
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk)
-                        mma_f16_ta(d, kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, kk || C::kF32 ? 1u : 0u);
+                        mma_f16_ta(d, C::kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, kk || C::kF32 ? 1u : 0u);
                     commit_elect(&empty[sk]);
                     commit_elect(&sfull[buf]);
                 }
-                if (i > 0) {
-                    // tile i - 1's values: the stage before K(i) (the last one: before the end)
-                    const uint32_t v = vslot;
-                    const bool first = i - 1 < C::kNS;
+                if (i >= C::kAhead) {
+                    const int j = i - C::kAhead;
                     // the last segment's O is read by now, or will be soon
-                    if (i == 1 && segs > 1 && !(ok = warp_wait_fast(oready, segs & 1u, a.status))) break;
-                    if (!(ok = issue_pv(tile + i - 1, v % C::kStages, v / C::kStages, first))) break;
+                    if (j == 0 && segs > 1 && !(ok = warp_wait(oready, segs & 1u, a.status))) break;
+                    ok = issue_pv(tile + j, j < C::kNS);
                 }
-                vslot = st + 1;
-                if (i < n) st += 2;
             }
             tile += n;
         }
@@ -656,8 +675,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         const int wg = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         uint8_t *scratch = smem + C::kOffScratch + warp * 4096;
-        float *qmax = reinterpret_cast<float *>(ml + 2 * kM);   // F32: [warpgroup][row] largest |q| of its columns
-        uint32_t tile = 0, st = 0;              // before the segment
+        float *qmax = reinterpret_cast<float *>(ml + 2 * kM);   // F32: largest |q| of a warp's rows and columns
+        uint32_t tile = 0;                      // before the segment
         uint32_t pv0 = 0, pv1 = 0;              // products of each stream so far
         bool ok = true;
         auto soft_bar = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kSoftWarps) : "memory"); };
@@ -688,25 +707,16 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 r += kRpi;
                 h += kRpi;
                 if (g.prefix)
+#pragma unroll 1
                     while (h >= a.group) h -= a.group, ++b;
             }
         };
-        // F32: the rows' largest |q| in a batch, for the lane that owns the row
+        // F32: the largest |q| of the warp's rows in a batch
         auto q_top = [&](const uint4 (&v)[kBatch * kIt], float top) {
 #pragma unroll
-            for (int i = 0; i < kIt; ++i) {
-                float m = 0.0f;
-#pragma unroll
-                for (int c = 0; c < kBatch; ++c) {
-                    const uint4 x = v[c * kIt + i];
-                    m = fmaxf(m, fmaxf(fmaxf(fabsf(__uint_as_float(x.x)), fabsf(__uint_as_float(x.y))),
-                                       fmaxf(fabsf(__uint_as_float(x.z)), fabsf(__uint_as_float(x.w)))));
-                }
-#pragma unroll
-                for (int o = 1; o < kLpr; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float x = __shfl_sync(0xffffffffu, m, (lane % kRpi) * kLpr);
-                if (lane / kRpi == i) top = fmaxf(top, x);
-            }
+            for (int i = 0; i < kBatch * kIt; ++i)
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(v[i].x)), fabsf(__uint_as_float(v[i].y))),
+                                       fmaxf(fabsf(__uint_as_float(v[i].z)), fabsf(__uint_as_float(v[i].w)))));
             return top;
         };
         auto q_store = [&](int c0, const uint4 (&v)[kBatch * kIt], float qs) {
@@ -732,7 +742,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         hi[4 * u] = x.x ^ f, hi[4 * u + 1] = x.y ^ f, hi[4 * u + 2] = x.z ^ f, hi[4 * u + 3] = x.w ^ f;
                     }
                 }
-                const uint32_t col = lanes + kColQ + 16 * ((c0 + c) * C::kNS + wg);
+                const uint32_t col = lanes + C::kColQ + 16 * ((c0 + c) * C::kNS + wg);
                 tmem_st16(col, hi);
                 if constexpr (C::kF32) tmem_st16(col + HD / 2, lo);
                 __syncwarp();
@@ -748,25 +758,29 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             if constexpr (C::kF32) {
                 if (quarter * 32 >= g.rows || q_idle) return;
                 float top = q_top(qv, 0.0f);
+#pragma unroll 1
                 for (int c = kBatch; c < kChunks; c += kBatch) {
                     uint4 v[kBatch * kIt];
                     q_load(g, c, v);
                     top = q_top(v, top);
                 }
-                qmax[wg * kM + row] = top;
+                top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                if (lane == 0) qmax[warp] = top;
             }
         };
-        // .. and after it: Q written, the score factor of this thread's row returned
+        // .. and after it: Q written (F32: under the power of two of its 32 rows), the
+        // rows' score factor returned
         auto q_finish = [&](const Seg &g) -> float {
             float qs = a.sign, cq = a.c;
             if (quarter * 32 < g.rows) {
                 if constexpr (C::kF32) {
-                    const float top = C::kNS == 2 && HD > 32 ? fmaxf(qmax[row], qmax[kM + row]) : qmax[row];
+                    const float top = C::kNS == 2 && HD > 32 ? fmaxf(qmax[quarter], qmax[4 + quarter]) : qmax[quarter];
                     const int e = part_exponent(top);
                     qs = a.sign * pow2(-e);
                     cq = a.c * pow2(e);
                 }
                 if (!q_idle) q_store(0, qv, qs);
+#pragma unroll 1
                 for (int c = kBatch; c < kChunks; c += kBatch) {
                     uint4 v[kBatch * kIt];
                     q_load(g, c, v);
@@ -789,63 +803,64 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             if constexpr (C::kF32) soft_bar();
             cq = q_finish(s);
         }
+#pragma unroll 1
         while (have) {
             const int n = s.j1 - s.j0;
             const bool active = quarter * 32 < s.rows;    // a row of this warp belongs to the unit
             const bool mine = row < s.rows;
             // ---- this warpgroup's tiles ----------------------------------------------------------
             float mref = 0.0f, l = 0.0f;
-            bool any = false, had = false;
+            bool any = false;
+            bool had = false;                             // a tile of the segment was this warpgroup's
             float *score = nullptr;
             if (a.add_weights && !s.prefix && s.dv == 0 && mine)
                 score = a.score + ((size_t)s.b * a.n_head + (size_t)s.g * a.group + s.m * kM + row) * a.pitch;
+#pragma unroll 1
             for (int i = 0; i < n; ++i) {
-                const uint32_t t = tile + i, buf = t & 1u;
-                const uint32_t stream = C::kNS == 2 ? buf : 0;
-                const uint32_t sv = st + 2 * i + 1;             // the stage of the tile's values
-                if (C::kNS == 1 || (int)buf == wg) {
-                    // This stream's last product complete.  With two streams S(t)
-                    // complete already means it (it was issued first); with one
-                    // stream every product is waited for, so that the barrier
-                    // is never two phases ahead of a wait.
-                    bool waited = C::kNS == 2 || pv0 == 0;
+                const uint32_t t = tile + i, buf = t % C::kBufs;
+                const uint32_t stream = C::kNS == 2 ? t & 1u : 0;
+                const uint32_t sv = 2 * t + 1;                  // the stage of the tile's values
+                if (C::kNS == 1 || (int)stream == wg) {
+                    // This stream's last product complete.  Every product is waited
+                    // for, before the weights of the next are handed over, so that
+                    // the barrier is never two phases away from a wait, where its
+                    // parity would mislead.
+                    const uint32_t done = stream ? pv1 : pv0;
+                    bool waited = done == 0;
                     auto wait_pv = [&]() {
                         if (waited) return;
-                        ok = ok && warp_wait_fast(&ofull[0], (pv0 - 1) & 1u, a.status);
+                        ok = ok && warp_wait(&ofull[stream], (done - 1) & 1u, a.status);
                         waited = true;
                         tc_after();
                     };
                     had = true;
                     const int valid = s.n - (s.j0 + i) * kTile;     // of the tile's 64 rows
-                    ok = ok && warp_wait_fast(&sfull[buf], (t >> 1) & 1u, a.status);
+                    ok = ok && warp_wait(&sfull[buf], (t / C::kBufs) & 1u, a.status);
                     tc_after();
                     if constexpr (!C::kF32) {
                         // stale rows behind a sequence's end may hold anything, NaN too,
                         // and 0 x NaN is NaN: the values' tile gets zeros there
                         if (!s.prefix && valid < kTile) {
-                            ok = ok && warp_wait_fast(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
+                            ok = ok && warp_wait(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
                             uint8_t *v = smem + (sv % C::kStages) * C::kStage;
                             constexpr int kU = C::kSubW * 2 / 16;
                             const int units = (kTile - valid) * kU;
 #pragma unroll
                             for (int c = 0; c < HD / C::kSubW; ++c)
+#pragma unroll 1
                                 for (int u = quarter * 32 + lane; u < units; u += 128)
                                     *reinterpret_cast<uint4 *>(v + c * C::kSub + valid * C::kSubW * 2 + u * 16) =
                                         make_uint4(0, 0, 0, 0);
                             fence_async();
                         }
                     } else {
-                        ok = ok && warp_wait_fast(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
+                        ok = ok && warp_wait(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
                     }
                     if (active && ok) {
-                        const uint32_t sc = lanes + kColS + buf * kTile;
+                        const uint32_t sc = lanes + C::kColS + buf * kTile;
                         const float *sd = side + (t % kSide) * 16;
                         // never 0: -inf (a row past the end) times it has to stay -inf
                         auto factor = [&](int g) { return fmaxf(sd[g] * cq, 1e-37f); };
-                        // 16 bits: the tile's 64 scores stay in registers; F32, with fewer of
-                        // them, reads each half again for its weights
-                        constexpr int kHeld = C::kF32 ? 32 : 64;
-                        float x[kHeld];
                         auto past_end = [&](float *y, int j0, int nj) {
                             if (valid < kTile) {
 #pragma unroll
@@ -854,12 +869,16 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                             }
                         };
                         float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                        if constexpr (C::kF32) {
-#pragma unroll
-                            for (int h = 1; h >= 0; --h) {
-                                tmem_ld32_nowait(sc + 32 * h, x);
-                                tmem_wait_ld();
-                                past_end(x, 32 * h, 32);
+                        // Loops over 16 or 32 scores, read again for the weights: a tile held in
+                        // registers needs everything unrolled, and fetching that much code once
+                        // per tile costs more than the reads
+#pragma unroll 1
+                        for (int h = 0; h < 2; ++h) {
+                            float x[32];
+                            tmem_ld32_nowait(sc + 32 * h, x);
+                            tmem_wait_ld();
+                            past_end(x, 32 * h, 32);
+                            if constexpr (C::kF32) {
 #pragma unroll
                                 for (int g = 0; g < 4; ++g) {
                                     const float f = factor(4 * h + g), e = sd[8 + 4 * h + g];
@@ -867,27 +886,17 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                                     for (int j = 0; j < 8; ++j)
                                         top4[j & 3] = fmaxf(top4[j & 3], fmaf(x[8 * g + j], f, e));
                                 }
-                                if (score) {
-                                    float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile + 32 * h);
+                            } else {
 #pragma unroll
-                                    for (int j = 0; j < 32; j += 4) {
-                                        const float f = factor(4 * h + (j >> 3));
-                                        o[j >> 2] = make_float4(x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f);
-                                    }
-                                }
+                                for (int j = 0; j < 32; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
                             }
-                        } else {
-                            tmem_ld32_nowait(sc, x);
-                            tmem_ld32_nowait(sc + 32, x + 32);
-                            tmem_wait_ld();
-                            past_end(x, 0, 64);
-#pragma unroll
-                            for (int j = 0; j < kTile; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
                             if (score) {
-                                float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile);
+                                float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile + 32 * h);
 #pragma unroll
-                                for (int j = 0; j < kTile; j += 4)
-                                    o[j >> 2] = make_float4(x[j] * cq, x[j + 1] * cq, x[j + 2] * cq, x[j + 3] * cq);
+                                for (int j = 0; j < 32; j += 4) {
+                                    const float f = C::kF32 ? factor(4 * h + (j >> 3)) : cq;
+                                    o[j >> 2] = make_float4(x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f);
+                                }
                             }
                         }
                         float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
@@ -913,18 +922,13 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                             }
                         }
                         // ---- weights -------------------------------------------------------------------
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t w[32];
+                        auto weigh = [&](float *x, int kk) {     // scores 16 kk ..: their weights in their place
+                            uint32_t w[16];
+                            past_end(x, 16 * kk, 16);
                             if constexpr (C::kF32) {
-                                if (h == 1) {       // the first half is still there
-                                    tmem_ld32_nowait(sc + 32, x);
-                                    tmem_wait_ld();
-                                    past_end(x, 32, 32);
-                                }
 #pragma unroll
-                                for (int g = 0; g < 4; ++g) {
-                                    const float ev = sd[8 + 4 * h + g], f = factor(4 * h + g), e = ev - mref;
+                                for (int g = 0; g < 2; ++g) {
+                                    const float ev = sd[8 + 2 * kk + g], f = factor(2 * kk + g), e = ev - mref;
                                     float sum = 0.0f;
 #pragma unroll
                                     for (int j = 0; j < 8; j += 2) {
@@ -932,23 +936,33 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                                         const float p1 = ex2(fmaf(x[8 * g + j + 1], f, e));
                                         sum += p0 + p1;
                                         const int o = 4 * g + (j >> 1);
-                                        w[o] = split2<__half>(p0, p1, w[16 + o]);
+                                        w[o] = split2<__half>(p0, p1, w[8 + o]);
                                     }
                                     l = fmaf(sum, pow2(-(int)ev), l);
                                 }
                             } else {
                                 float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
-                                for (int j = 0; j < 32; j += 2) {
-                                    const float p0 = ex2(fmaf(x[32 * h + j], cq, -mref));
-                                    const float p1 = ex2(fmaf(x[32 * h + j + 1], cq, -mref));
+                                for (int j = 0; j < 16; j += 2) {
+                                    const float p0 = ex2(fmaf(x[j], cq, -mref)), p1 = ex2(fmaf(x[j + 1], cq, -mref));
                                     l0 += p0;
                                     l1 += p1;
-                                    w[j >> 1] = split2<T>(p0, p1, w[16 + (j >> 1)]);
+                                    w[j >> 1] = split2<T>(p0, p1, w[8 + (j >> 1)]);
                                 }
                                 l += l0 + l1;
                             }
-                            tmem_st32(sc + 32 * h, w);
+                            tmem_st16(sc + 16 * kk, w);
+                        };
+                        float xa[16], xb[16];
+                        tmem_ld16_nowait(sc, xa);
+#pragma unroll 1
+                        for (int kk = 0; kk < 4; kk += 2) {
+                            tmem_wait_ld();
+                            tmem_ld16_nowait(sc + 16 * kk + 16, xb);
+                            weigh(xa, kk);
+                            tmem_wait_ld();
+                            if (kk == 0) tmem_ld16_nowait(sc + 32, xa);
+                            weigh(xb, kk + 1);
                         }
                         tmem_wait_st();
                         any = true;
@@ -973,7 +987,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             if (nhave) q_begin(nx);
             if (had) {
                 const uint32_t k = C::kNS == 2 ? wg : 0;
-                ok = ok && warp_wait_fast(&ofull[k], ((k ? pv1 : pv0) - 1) & 1u, a.status);
+                ok = ok && warp_wait(&ofull[k], ((k ? pv1 : pv0) - 1) & 1u, a.status);
             }
             ml[wg * kM + row] = make_float2(mref, l);
             if (nhave) q_share(nx);
@@ -1009,6 +1023,15 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         o[k] = has0 ? o[k] * f0 : 0.0f;
                         if (C::kNS == 2 && has1) o[k] = fmaf(v[k], f1, o[k]);
                     }
+                    if (live <= 8) {      // a few rows: each lane its own
+                        if (lane < live) {
+#pragma unroll
+                            for (int u = 0; u < kOl; ++u)
+                                *reinterpret_cast<float4 *>(po + (size_t)lane * C::kDV + c + 4 * u) =
+                                    make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                        }
+                        continue;
+                    }
 #pragma unroll
                     for (int u = 0; u < kOl; ++u)
                         *reinterpret_cast<float4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4)) =
@@ -1027,7 +1050,6 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(oready);
             tile += n;
-            st += 2 * n;
             s = nx;
             have = nhave;
             cq = cn;

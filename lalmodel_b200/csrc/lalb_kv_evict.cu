@@ -37,7 +37,7 @@ constexpr size_t kKeyBytesMax = 180 * 1024;   // keys of up to 46080 rows of a C
 constexpr int kMaxCluster = 4;
 constexpr int kRowsPerCta = 8192;             // fewer are not worth another CTA
 constexpr int kMoveThreads = 256;
-constexpr int kMoveUnroll = 4;
+constexpr int kMoveUnroll = 2;                // 16-byte pieces in flight per thread (4 and 8: 2 and 6 us more of 31)
 constexpr int kMoveFill = 16;                 // blocks per SM
 
 struct EvictArgs {
