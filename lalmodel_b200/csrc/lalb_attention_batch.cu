@@ -89,8 +89,8 @@ struct Cfg {
     // Registers a thread: the launch's even share, and the split of it (the
     // softmax holds a tile's scores and weights; at the even share it spills)
     static constexpr int kEven = kThreads == 512 ? 128 : kThreads == 384 ? 168 : 248;
-    static constexpr int kSoftRegs = kF32 ? (kNS == 2 ? 152 : 232) : kNS == 2 ? 208 : 0;   // 0: no split
-    static constexpr int kOtherRegs = kF32 ? (kNS == 2 ? 104 : 136) : 88;
+    static constexpr int kSoftRegs = kF32 ? (kNS == 2 ? 152 : 232) : kNS == 2 ? 200 : 0;   // 0: no split
+    static constexpr int kOtherRegs = kF32 ? (kNS == 2 ? 104 : 136) : 104;
     static_assert(kSoftRegs == 0 || kSoftRegs * kSoftWarps + kOtherRegs * kOtherWarps <=
                                         kEven * (kSoftWarps + kOtherWarps),
                   "the split is no more than the block was launched with");
@@ -103,7 +103,7 @@ struct Cfg {
     static constexpr uint32_t kSub = kTile * kSubW * 2;               // its bytes
     static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
     static constexpr uint32_t kOffMl = kOffScratch + kSoftWarps * 4096;
-    static constexpr uint32_t kOffSide = kOffMl + 2 * kM * 8 + (kF32 ? 32 : 0);   // ml, and F32's qmax
+    static constexpr uint32_t kOffSide = kOffMl + 2 * (2 * kM * 8 + 32);   // ml and qmax, of two segments
     static constexpr uint32_t kOffBar = kOffSide + kSide * 16 * 4;
     static constexpr uint32_t kSmem = 1024 + kOffBar + 512;
     static_assert(kSmem <= 232448, "fits the 227 KB opt-in shared memory");
@@ -301,19 +301,19 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// x0, x1 as two 16-bit parts each: returns the pair of high parts, lo the rest.
+// x0, x1 as two 16-bit parts each: returns the pair of high parts, lo the
+// rest.  The high part is x cut off (not rounded) to 11 or 8 bits, so that
+// the rest is one mask and one subtraction; with the rest rounded to as many
+// bits again the two are within 2^-22 (fp16) or 2^-16 (bf16) of x.
 template <class H>
-__device__ __forceinline__ uint32_t split2(float x0, float x1, uint32_t &lo) {
-    const uint32_t h = pack2<H>(x0, x1);
-    float h0, h1;
-    if constexpr (std::is_same<H, __half>::value) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-        h0 = f.x, h1 = f.y;
-    } else {
-        h0 = __uint_as_float(h << 16), h1 = __uint_as_float(h & 0xffff0000u);
-    }
-    lo = pack2<H>(x0 - h0, x1 - h1);
-    return h;
+__device__ __forceinline__ uint32_t split2(float2 x, uint32_t &lo) {
+    constexpr uint32_t kKeep = std::is_same<H, __half>::value ? 0xffffe000u : 0xffff0000u;
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & kKeep),
+                                 __uint_as_float(__float_as_uint(x.y) & kKeep));
+    const float2 r = __fadd2_rn(x, make_float2(-h.x, -h.y));
+    lo = pack2<H>(r.x, r.y);
+    if constexpr (std::is_same<H, __half>::value) return pack2<H>(h.x, h.y);
+    return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);   // bf16: the upper halves
 }
 
 // Exponent e, 2^e the power of two that v 2^-e puts |v| <= amax below 2^15
@@ -383,8 +383,8 @@ struct RowLoad {
         for (int i = 0; i < kN; ++i) {
             const int r = r0 + i / kVec * kPer + rr, c = cc + (i % kVec) * 4 * kLanes;
             uint2 hi, lo;
-            hi.x = split2<__half>(x[i].x * scale, x[i].y * scale, lo.x);
-            hi.y = split2<__half>(x[i].z * scale, x[i].w * scale, lo.y);
+            hi.x = split2<__half>(make_float2(x[i].x * scale, x[i].y * scale), lo.x);
+            hi.y = split2<__half>(make_float2(x[i].z * scale, x[i].w * scale), lo.y);
             const int unit = (c % W) >> 3;
             const int sw = W == 64 ? unit ^ (r & 7) : unit ^ ((r >> 1) & 3);
             const uint32_t off = (uint32_t)(c / W) * (kTile * W * 2) + r * (W * 2) + sw * 16 + (c & 4) * 2;
@@ -402,7 +402,6 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     using C = Cfg<T, HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    float2 *ml = reinterpret_cast<float2 *>(smem + C::kOffMl);        // [stream][row]
     float *side = reinterpret_cast<float *>(smem + C::kOffSide);      // [tile % kSide][K 8, V 8]
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
     uint64_t *empty = full + C::kStages;
@@ -547,22 +546,36 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     static_cast<const float *>(s.prefix ? a.pv : a.v) + seq + (size_t)s.g * HD + s.dv * C::kDV;
 #pragma unroll 1
                 for (int j = s.j0; j < s.j1 && ok; ++j, ++tile) {
+                    if constexpr (C::kDV == HD) {       // one loop, half of the code
 #pragma unroll 1
-                    for (int g = turn; g < 8; g += C::kLoadWarps) {
-                        RowLoad<HD> x;
-                        group(x, kb, j, s.n, g);
-                        finish(x, g, false);
-                    }
-                    ++st;
-                    turn = (turn + 6) % 7;          // 8 groups on: -8 = 6 mod 7
+                        for (int kv = 0; kv < 2; ++kv) {
 #pragma unroll 1
-                    for (int g = turn; g < 8; g += C::kLoadWarps) {
-                        RowLoad<C::kDV> x;
-                        group(x, vb, j, s.n, g);
-                        finish(x, g, true);
+                            for (int g = turn; g < 8; g += C::kLoadWarps) {
+                                RowLoad<HD> x;
+                                group(x, kv ? vb : kb, j, s.n, g);
+                                finish(x, g, kv);
+                            }
+                            ++st;
+                            turn = (turn + 6) % 7;      // 8 groups on: -8 = 6 mod 7
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int g = turn; g < 8; g += C::kLoadWarps) {
+                            RowLoad<HD> x;
+                            group(x, kb, j, s.n, g);
+                            finish(x, g, false);
+                        }
+                        ++st;
+                        turn = (turn + 6) % 7;
+#pragma unroll 1
+                        for (int g = turn; g < 8; g += C::kLoadWarps) {
+                            RowLoad<C::kDV> x;
+                            group(x, vb, j, s.n, g);
+                            finish(x, g, true);
+                        }
+                        ++st;
+                        turn = (turn + 6) % 7;
                     }
-                    ++st;
-                    turn = (turn + 6) % 7;
                 }
             }
         } else if (lane == 0) {
@@ -675,7 +688,11 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         const int wg = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         uint8_t *scratch = smem + C::kOffScratch + warp * 4096;
-        float *qmax = reinterpret_cast<float *>(ml + 2 * kM);   // F32: largest |q| of a warp's rows and columns
+        // Two of each, taken in turn: a warpgroup without a tile in a segment may
+        // be at the next boundary while the other still reads this one's.
+        float2 *ml = reinterpret_cast<float2 *>(smem + C::kOffMl);    // [stream][row]: (m, l)
+        float *qmax = reinterpret_cast<float *>(ml + 2 * 2 * kM);     // F32: largest |q| of a warp's rows and columns
+        uint32_t turn = 0;
         uint32_t tile = 0;                      // before the segment
         uint32_t pv0 = 0, pv1 = 0;              // products of each stream so far
         bool ok = true;
@@ -733,9 +750,10 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 for (int u = 0; u < kLpr; ++u) {
                     const uint4 x = *reinterpret_cast<const uint4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4));
                     if constexpr (C::kF32) {
-                        hi[2 * u] = split2<__half>(__uint_as_float(x.x) * qs, __uint_as_float(x.y) * qs, lo[2 * u]);
-                        hi[2 * u + 1] =
-                            split2<__half>(__uint_as_float(x.z) * qs, __uint_as_float(x.w) * qs, lo[2 * u + 1]);
+                        hi[2 * u] = split2<__half>(
+                            make_float2(__uint_as_float(x.x) * qs, __uint_as_float(x.y) * qs), lo[2 * u]);
+                        hi[2 * u + 1] = split2<__half>(
+                            make_float2(__uint_as_float(x.z) * qs, __uint_as_float(x.w) * qs), lo[2 * u + 1]);
                     } else {
                         // a negative scale turns the queries' signs
                         const uint32_t f = qs < 0.0f ? 0x80008000u : 0u;
@@ -765,7 +783,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     top = q_top(v, top);
                 }
                 top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                if (lane == 0) qmax[warp] = top;
+                if (lane == 0) qmax[turn * 8 + warp] = top;
             }
         };
         // .. and after it: Q written (F32: under the power of two of its 32 rows), the
@@ -774,7 +792,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             float qs = a.sign, cq = a.c;
             if (quarter * 32 < g.rows) {
                 if constexpr (C::kF32) {
-                    const float top = C::kNS == 2 && HD > 32 ? fmaxf(qmax[quarter], qmax[4 + quarter]) : qmax[quarter];
+                    const float *qm = qmax + turn * 8 + quarter;
+                    const float top = C::kNS == 2 && HD > 32 ? fmaxf(qm[0], qm[4]) : qm[0];
                     const int e = part_exponent(top);
                     qs = a.sign * pow2(-e);
                     cq = a.c * pow2(e);
@@ -795,25 +814,100 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         };
 
         Seg nx;
-        bool have = walk.template next<C::kNDV>(a, list, s);
-        float cq = 0.0f;
-        if (have) {
-            q_begin(s);
-            q_share(s);
-            if constexpr (C::kF32) soft_bar();
-            cq = q_finish(s);
-        }
+        int n = 0;                               // the segment's tiles
+        bool have = false, had = false;          // a segment is open; one of its tiles was this warpgroup's
+        bool active = false;                     // a row of this warp belongs to its unit
+        float cq = 0.0f, mref = 0.0f, l = 0.0f;
 #pragma unroll 1
-        while (have) {
-            const int n = s.j1 - s.j0;
-            const bool active = quarter * 32 < s.rows;    // a row of this warp belongs to the unit
-            const bool mine = row < s.rows;
+        for (;;) {
+            // ---- from one segment to the next ------------------------------------------------------
+            // The next segment's Q is on its way while the last products run.  Each
+            // warpgroup waits for its own stream's last one; past the barrier every
+            // product is complete, Q and the score buffers are free, and the next
+            // scores can start while O is read.
+            const bool nhave = walk.template next<C::kNDV>(a, list, nx);
+            if (nhave) q_begin(nx);
+            if (had) {
+                const uint32_t k = C::kNS == 2 ? wg : 0;
+                ok = ok && warp_wait(&ofull[k], ((k ? pv1 : pv0) - 1) & 1u, a.status);
+            }
+            ml[turn * 2 * kM + wg * kM + row] = make_float2(mref, l);
+            if (nhave) q_share(nx);
+            tc_before();
+            soft_bar();
+            tc_after();
+            const float2 *mlt = ml + turn * 2 * kM;
+            const float2 r0 = mlt[row], r1 = C::kNS == 2 ? mlt[kM + row] : make_float2(0.0f, 0.0f);
+            float cn = 0.0f;
+            if (nhave) cn = q_finish(nx);
+            turn ^= 1;
+            if (have) {
+                // a stream without a tile in this segment has nothing (the other has)
+                const bool has0 = C::kNS == 1 || n > 1 || (tile & 1u) == 0, has1 = C::kNS == 2 && (n > 1 || (tile & 1u) == 1);
+                const float m = has0 && has1 ? fmaxf(r0.x, r1.x) : has0 ? r0.x : r1.x;
+                const float f0 = has0 ? ex2(r0.x - m) : 0.0f, f1 = has1 ? ex2(r1.x - m) : 0.0f;
+                if (active && ok) {
+                    const int rows = s.prefix ? a.rows_p : a.rows_o;
+                    const size_t first = (size_t)s.slot * rows + quarter * 32;
+                    float *po = (s.prefix ? a.part_p : a.part_o) + first * C::kDV;
+                    float2 *pm = (s.prefix ? a.ml_p : a.ml_o) + first;
+                    const int live = min(32, s.rows - quarter * 32);
+                    if (wg == 0 && row < s.rows)
+                        pm[lane] = make_float2(m, (has0 ? r0.y * f0 : 0.0f) + (has1 ? r1.y * f1 : 0.0f));
+                    constexpr int kHalf = C::kDV / C::kNS, kP = 16;
+                    constexpr int kOl = kP / 4, kOr = 32 / kOl;      // lanes of a row's piece, rows per store
+                    const int olr = lane / kOl, olu = lane % kOl;
+#pragma unroll 1
+                    for (int c = wg * kHalf; c < (wg + 1) * kHalf; c += kP) {
+                        float o[kP], v[kP];
+                        tmem_ld16_nowait(lanes + C::kColO + c, o);
+                        if constexpr (C::kNS == 2) tmem_ld16_nowait(lanes + C::kColO + C::kDV + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < kP; ++k) {
+                            o[k] = has0 ? o[k] * f0 : 0.0f;
+                            if (C::kNS == 2 && has1) o[k] = fmaf(v[k], f1, o[k]);
+                        }
+                        if (live <= 8) {      // a few rows: each lane its own
+                            if (lane < live) {
+#pragma unroll
+                                for (int u = 0; u < kOl; ++u)
+                                    *reinterpret_cast<float4 *>(po + (size_t)lane * C::kDV + c + 4 * u) =
+                                        make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                            }
+                            continue;
+                        }
+#pragma unroll
+                        for (int u = 0; u < kOl; ++u)
+                            *reinterpret_cast<float4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4)) =
+                                make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                        __syncwarp();
+#pragma unroll
+                        for (int r = 0; r < 32; r += kOr)
+                            if (r + olr < live)
+                                *reinterpret_cast<float4 *>(po + (size_t)(r + olr) * C::kDV + c + 4 * olu) =
+                                    *reinterpret_cast<const float4 *>(scratch + (r + olr) * 128 +
+                                                                      ((olu ^ ((r + olr) & 7)) << 4));
+                        __syncwarp();
+                    }
+                }
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(oready);
+                tile += n;
+            }
+            if (!nhave) break;
             // ---- this warpgroup's tiles ----------------------------------------------------------
-            float mref = 0.0f, l = 0.0f;
+            s = nx;
+            have = true;
+            cq = cn;
+            n = s.j1 - s.j0;
+            active = quarter * 32 < s.rows;
+            mref = l = 0.0f;
             bool any = false;
-            bool had = false;                             // a tile of the segment was this warpgroup's
+            had = false;
             float *score = nullptr;
-            if (a.add_weights && !s.prefix && s.dv == 0 && mine)
+            if (a.add_weights && !s.prefix && s.dv == 0 && row < s.rows)
                 score = a.score + ((size_t)s.b * a.n_head + (size_t)s.g * a.group + s.m * kM + row) * a.pitch;
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
@@ -869,33 +963,50 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                             }
                         };
                         float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                        // Loops over 16 or 32 scores, read again for the weights: a tile held in
-                        // registers needs everything unrolled, and fetching that much code once
-                        // per tile costs more than the reads
-#pragma unroll 1
-                        for (int h = 0; h < 2; ++h) {
-                            float x[32];
-                            tmem_ld32_nowait(sc + 32 * h, x);
+                        // 16 bits: the tile's scores stay in registers.  F32: loops over 32
+                        // or 16 of them, read again for the weights: unrolled, its longer
+                        // code is fetched more slowly than the scores are read.
+                        constexpr int kHeld = C::kF32 ? 1 : kTile;
+                        float x[kHeld];
+                        if constexpr (!C::kF32) {
+                            tmem_ld32_nowait(sc, x);
+                            tmem_ld32_nowait(sc + 32, x + 32);
                             tmem_wait_ld();
-                            past_end(x, 32 * h, 32);
-                            if constexpr (C::kF32) {
+                            past_end(x, 0, kTile);
+#pragma unroll
+                            for (int j = 0; j < kTile; j += 8)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) top4[q] = fmaxf(top4[q], fmaxf(x[j + q], x[j + 4 + q]));
+                            if (score) {
+                                float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile);
+#pragma unroll
+                                for (int j = 0; j < kTile; j += 4)
+                                    o[j >> 2] = make_float4(x[j] * cq, x[j + 1] * cq, x[j + 2] * cq, x[j + 3] * cq);
+                            }
+                        } else {
+#pragma unroll 1
+                            for (int h = 0; h < 2; ++h) {
+                                float y[32];
+                                tmem_ld32_nowait(sc + 32 * h, y);
+                                tmem_wait_ld();
+                                past_end(y, 32 * h, 32);
 #pragma unroll
                                 for (int g = 0; g < 4; ++g) {
                                     const float f = factor(4 * h + g), e = sd[8 + 4 * h + g];
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j)
-                                        top4[j & 3] = fmaxf(top4[j & 3], fmaf(x[8 * g + j], f, e));
+                                    for (int j = 0; j < 8; j += 2) {
+                                        const float2 v = __ffma2_rn(make_float2(y[8 * g + j], y[8 * g + j + 1]),
+                                                                    make_float2(f, f), make_float2(e, e));
+                                        top4[j >> 1] = fmaxf(top4[j >> 1], fmaxf(v.x, v.y));
+                                    }
                                 }
-                            } else {
+                                if (score) {
+                                    float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile + 32 * h);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
-                            }
-                            if (score) {
-                                float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile + 32 * h);
-#pragma unroll
-                                for (int j = 0; j < 32; j += 4) {
-                                    const float f = C::kF32 ? factor(4 * h + (j >> 3)) : cq;
-                                    o[j >> 2] = make_float4(x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f);
+                                    for (int j = 0; j < 32; j += 4) {
+                                        const float f = factor(4 * h + (j >> 3));
+                                        o[j >> 2] = make_float4(y[j] * f, y[j + 1] * f, y[j + 2] * f, y[j + 3] * f);
+                                    }
                                 }
                             }
                         }
@@ -922,47 +1033,52 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                             }
                         }
                         // ---- weights -------------------------------------------------------------------
-                        auto weigh = [&](float *x, int kk) {     // scores 16 kk ..: their weights in their place
-                            uint32_t w[16];
-                            past_end(x, 16 * kk, 16);
-                            if constexpr (C::kF32) {
+                        // 16 scores and their weights in their place: eight columns of high
+                        // parts, eight of the rest
+                        float2 sum2 = make_float2(0.0f, 0.0f);
+                        auto weigh8 = [&](const float *y, float f, float e, uint32_t *hi, uint32_t *lo) {
+#pragma unroll
+                            for (int j = 0; j < 8; j += 2) {
+                                const float2 v =
+                                    __ffma2_rn(make_float2(y[j], y[j + 1]), make_float2(f, f), make_float2(e, e));
+                                const float2 p = make_float2(ex2(v.x), ex2(v.y));
+                                sum2 = __fadd2_rn(sum2, p);
+                                hi[j >> 1] = split2<typename std::conditional<C::kF32, __half, T>::type>(p, lo[j >> 1]);
+                            }
+                        };
+                        if constexpr (C::kF32) {
+                            auto weigh = [&](float *y, int kk) {
+                                uint32_t w[16];
+                                past_end(y, 16 * kk, 16);
 #pragma unroll
                                 for (int g = 0; g < 2; ++g) {
-                                    const float ev = sd[8 + 2 * kk + g], f = factor(2 * kk + g), e = ev - mref;
-                                    float sum = 0.0f;
-#pragma unroll
-                                    for (int j = 0; j < 8; j += 2) {
-                                        const float p0 = ex2(fmaf(x[8 * g + j], f, e));
-                                        const float p1 = ex2(fmaf(x[8 * g + j + 1], f, e));
-                                        sum += p0 + p1;
-                                        const int o = 4 * g + (j >> 1);
-                                        w[o] = split2<__half>(p0, p1, w[8 + o]);
-                                    }
-                                    l = fmaf(sum, pow2(-(int)ev), l);
+                                    const float ev = sd[8 + 2 * kk + g];
+                                    sum2 = make_float2(0.0f, 0.0f);
+                                    weigh8(y + 8 * g, factor(2 * kk + g), ev - mref, w + 4 * g, w + 8 + 4 * g);
+                                    l = fmaf(sum2.x + sum2.y, pow2(-(int)ev), l);
                                 }
-                            } else {
-                                float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-                                for (int j = 0; j < 16; j += 2) {
-                                    const float p0 = ex2(fmaf(x[j], cq, -mref)), p1 = ex2(fmaf(x[j + 1], cq, -mref));
-                                    l0 += p0;
-                                    l1 += p1;
-                                    w[j >> 1] = split2<T>(p0, p1, w[8 + (j >> 1)]);
-                                }
-                                l += l0 + l1;
-                            }
-                            tmem_st16(sc + 16 * kk, w);
-                        };
-                        float xa[16], xb[16];
-                        tmem_ld16_nowait(sc, xa);
+                                tmem_st16(sc + 16 * kk, w);
+                            };
+                            float xa[16], xb[16];
+                            tmem_ld16_nowait(sc, xa);
 #pragma unroll 1
-                        for (int kk = 0; kk < 4; kk += 2) {
-                            tmem_wait_ld();
-                            tmem_ld16_nowait(sc + 16 * kk + 16, xb);
-                            weigh(xa, kk);
-                            tmem_wait_ld();
-                            if (kk == 0) tmem_ld16_nowait(sc + 32, xa);
-                            weigh(xb, kk + 1);
+                            for (int kk = 0; kk < 4; kk += 2) {
+                                tmem_wait_ld();
+                                tmem_ld16_nowait(sc + 16 * kk + 16, xb);
+                                weigh(xa, kk);
+                                tmem_wait_ld();
+                                if (kk == 0) tmem_ld16_nowait(sc + 32, xa);
+                                weigh(xb, kk + 1);
+                            }
+                        } else {
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                uint32_t w[16];
+                                weigh8(x + 16 * kk, cq, -mref, w, w + 8);
+                                weigh8(x + 16 * kk + 8, cq, -mref, w + 4, w + 12);
+                                tmem_st16(sc + 16 * kk, w);
+                            }
+                            l += sum2.x + sum2.y;
                         }
                         tmem_wait_st();
                         any = true;
@@ -977,82 +1093,6 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 else
                     ++pv0;
             }
-
-            // ---- the segment's end -----------------------------------------------------------------
-            // The next segment's Q is on its way while the last products run.  Each
-            // warpgroup waits for its own stream's last one; past the barrier every
-            // product is complete, Q and the score buffers are free, and the next
-            // scores can start while O is read.
-            const bool nhave = walk.template next<C::kNDV>(a, list, nx);
-            if (nhave) q_begin(nx);
-            if (had) {
-                const uint32_t k = C::kNS == 2 ? wg : 0;
-                ok = ok && warp_wait(&ofull[k], ((k ? pv1 : pv0) - 1) & 1u, a.status);
-            }
-            ml[wg * kM + row] = make_float2(mref, l);
-            if (nhave) q_share(nx);
-            tc_before();
-            soft_bar();
-            tc_after();
-            const float2 r0 = ml[row], r1 = C::kNS == 2 ? ml[kM + row] : make_float2(0.0f, 0.0f);
-            float cn = 0.0f;
-            if (nhave) cn = q_finish(nx);
-            // a stream without a tile in this segment has nothing (the other has)
-            const bool has0 = C::kNS == 1 || n > 1 || (tile & 1u) == 0, has1 = C::kNS == 2 && (n > 1 || (tile & 1u) == 1);
-            const float m = has0 && has1 ? fmaxf(r0.x, r1.x) : has0 ? r0.x : r1.x;
-            const float f0 = has0 ? ex2(r0.x - m) : 0.0f, f1 = has1 ? ex2(r1.x - m) : 0.0f;
-            if (active && ok) {
-                const int rows = s.prefix ? a.rows_p : a.rows_o;
-                const size_t first = (size_t)s.slot * rows + quarter * 32;
-                float *po = (s.prefix ? a.part_p : a.part_o) + first * C::kDV;
-                float2 *pm = (s.prefix ? a.ml_p : a.ml_o) + first;
-                const int live = min(32, s.rows - quarter * 32);
-                if (wg == 0 && mine)
-                    pm[lane] = make_float2(m, (has0 ? r0.y * f0 : 0.0f) + (has1 ? r1.y * f1 : 0.0f));
-                constexpr int kHalf = C::kDV / C::kNS, kP = 16;
-                constexpr int kOl = kP / 4, kOr = 32 / kOl;      // lanes of a row's piece, rows per store
-                const int olr = lane / kOl, olu = lane % kOl;
-#pragma unroll 1
-                for (int c = wg * kHalf; c < (wg + 1) * kHalf; c += kP) {
-                    float o[kP], v[kP];
-                    tmem_ld16_nowait(lanes + C::kColO + c, o);
-                    if constexpr (C::kNS == 2) tmem_ld16_nowait(lanes + C::kColO + C::kDV + c, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < kP; ++k) {
-                        o[k] = has0 ? o[k] * f0 : 0.0f;
-                        if (C::kNS == 2 && has1) o[k] = fmaf(v[k], f1, o[k]);
-                    }
-                    if (live <= 8) {      // a few rows: each lane its own
-                        if (lane < live) {
-#pragma unroll
-                            for (int u = 0; u < kOl; ++u)
-                                *reinterpret_cast<float4 *>(po + (size_t)lane * C::kDV + c + 4 * u) =
-                                    make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
-                        }
-                        continue;
-                    }
-#pragma unroll
-                    for (int u = 0; u < kOl; ++u)
-                        *reinterpret_cast<float4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-                            make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
-                    __syncwarp();
-#pragma unroll
-                    for (int r = 0; r < 32; r += kOr)
-                        if (r + olr < live)
-                            *reinterpret_cast<float4 *>(po + (size_t)(r + olr) * C::kDV + c + 4 * olu) =
-                                *reinterpret_cast<const float4 *>(scratch + (r + olr) * 128 +
-                                                                  ((olu ^ ((r + olr) & 7)) << 4));
-                    __syncwarp();
-                }
-            }
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(oready);
-            tile += n;
-            s = nx;
-            have = nhave;
-            cq = cn;
         }
     }
     __syncwarp();
