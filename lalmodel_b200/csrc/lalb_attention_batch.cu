@@ -517,64 +517,73 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         set_regs<C::kSoftRegs ? C::kOtherRegs : 0, false>();
         // ================================ loaders ===============================================
         if constexpr (C::kF32) {
-            // a stage is 8 groups of 8 rows; the groups go round the loader warps
-            const int w = warp - C::kSoftWarps - 1;
+            // A stage is 8 groups of 8 rows; the groups go round the loader warps:
+            // warp w has groups w, w + 7, w + 14, .. of the CTA's stages.
             const size_t pitch = (size_t)a.n_kv * HD;
-            uint32_t st = 0, tile = 0;     // stages and tiles so far
-            uint32_t turn = w;             // the first group of stage st that is this warp's
+            int k = warp - C::kSoftWarps - 1;            // the next group to look at
+            int t0 = 0, t1 = 0;                          // the segment's tiles, counted over the CTA
+            const float *kb = nullptr, *vb = nullptr;
             bool ok = true;
-            auto group = [&](auto &x, const float *base, int j, int n, int g) {
-                const size_t row = (size_t)j * kTile + 8 * g;
-                x.load(base + row * pitch, pitch, n - (int)row, lane);
+            struct Task {
+                const float *p;
+                int left, k;
             };
-            auto finish = [&](auto &x, int g, bool is_v) {
+            auto advance = [&](Task &t) -> bool {
+                const int tile = k >> 4;
+#pragma unroll 1
+                while (tile >= t1) {
+                    if (!walk.template next<C::kNDV>(a, list, s)) return false;
+                    t0 = t1;
+                    t1 += s.j1 - s.j0;
+                    const size_t seq = s.prefix ? 0 : (size_t)s.b * a.max_ctx * pitch;
+                    kb = static_cast<const float *>(s.prefix ? a.pk : a.k) + seq + (size_t)s.g * HD;
+                    vb = static_cast<const float *>(s.prefix ? a.pv : a.v) + seq + (size_t)s.g * HD + s.dv * C::kDV;
+                }
+                const int row = (s.j0 + tile - t0) * kTile + 8 * (k & 7);
+                t.p = ((k >> 3) & 1 ? vb : kb) + (size_t)row * pitch;
+                t.left = s.n - row;
+                t.k = k;
+                k += C::kLoadWarps;
+                return true;
+            };
+            auto finish = [&](const auto &x, int k) {
+                const uint32_t st = k >> 3, g = k & 7, slot = st % C::kStages, use = st / C::kStages;
                 const int e = x.exponent();
-                const uint32_t slot = st % C::kStages, use = st / C::kStages;
                 if (use > 0) ok = ok && warp_wait(&empty[slot], (use - 1) & 1u, a.status);
                 x.store(smem + slot * C::kStage, 8 * g, pow2(-e), lane);
                 // K: the factor that undoes the scaling; V: the exponent
-                if (lane == 0) side[(tile % kSide) * 16 + (is_v ? 8 : 0) + g] = is_v ? (float)e : pow2(e);
+                if (lane == 0) side[((st >> 1) % kSide) * 16 + (st & 1) * 8 + g] = st & 1 ? (float)e : pow2(e);
                 fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[slot]);
             };
+            Task t;
+            if constexpr (C::kDV == HD) {
+                // the next group's loads are in flight while this one is converted
+                RowLoad<HD> x;
+                bool more = advance(t);
+                if (more) x.load(t.p, pitch, t.left, lane);
 #pragma unroll 1
-            while (walk.template next<C::kNDV>(a, list, s)) {
-                const size_t seq = s.prefix ? 0 : (size_t)s.b * a.max_ctx * pitch;
-                const float *kb = static_cast<const float *>(s.prefix ? a.pk : a.k) + seq + (size_t)s.g * HD;
-                const float *vb =
-                    static_cast<const float *>(s.prefix ? a.pv : a.v) + seq + (size_t)s.g * HD + s.dv * C::kDV;
+                while (more && ok) {
+                    Task u;
+                    RowLoad<HD> y;
+                    more = advance(u);
+                    if (more) y.load(u.p, pitch, u.left, lane);
+                    finish(x, t.k);
+                    x = y;
+                    t = u;
+                }
+            } else {
 #pragma unroll 1
-                for (int j = s.j0; j < s.j1 && ok; ++j, ++tile) {
-                    if constexpr (C::kDV == HD) {       // one loop, half of the code
-#pragma unroll 1
-                        for (int kv = 0; kv < 2; ++kv) {
-#pragma unroll 1
-                            for (int g = turn; g < 8; g += C::kLoadWarps) {
-                                RowLoad<HD> x;
-                                group(x, kv ? vb : kb, j, s.n, g);
-                                finish(x, g, kv);
-                            }
-                            ++st;
-                            turn = (turn + 6) % 7;      // 8 groups on: -8 = 6 mod 7
-                        }
+                while (ok && advance(t)) {
+                    if ((t.k >> 3) & 1) {
+                        RowLoad<C::kDV> x;
+                        x.load(t.p, pitch, t.left, lane);
+                        finish(x, t.k);
                     } else {
-#pragma unroll 1
-                        for (int g = turn; g < 8; g += C::kLoadWarps) {
-                            RowLoad<HD> x;
-                            group(x, kb, j, s.n, g);
-                            finish(x, g, false);
-                        }
-                        ++st;
-                        turn = (turn + 6) % 7;
-#pragma unroll 1
-                        for (int g = turn; g < 8; g += C::kLoadWarps) {
-                            RowLoad<C::kDV> x;
-                            group(x, vb, j, s.n, g);
-                            finish(x, g, true);
-                        }
-                        ++st;
-                        turn = (turn + 6) % 7;
+                        RowLoad<HD> x;
+                        x.load(t.p, pitch, t.left, lane);
+                        finish(x, t.k);
                     }
                 }
             }
