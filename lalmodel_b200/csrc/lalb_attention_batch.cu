@@ -58,6 +58,8 @@ namespace {
 constexpr int kGrid = 148;           // one CTA per SM of a B200 (workspace sizes need no device)
 constexpr int kTile = 64;            // cache rows per tile
 constexpr int kM = 128;              // query rows per unit
+constexpr int kPad = 3;              // list places a unit takes beside its tiles: what its segment's ends cost
+constexpr int kLens = 512;           // sequences whose lengths a CTA keeps in shared memory
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (loaders run at most 5 ahead)
 constexpr float kShift = 6.0f;       // weights up to 2^6 at the reference maximum, 2^14 before a rescale
 constexpr float kGrow = 8.0f;        // growth of a row's maximum that is left in place
@@ -104,7 +106,8 @@ struct Cfg {
     static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
     static constexpr uint32_t kOffMl = kOffScratch + kSoftWarps * 4096;
     static constexpr uint32_t kOffSide = kOffMl + 2 * (2 * kM * 8 + 32);   // ml and qmax, of two segments
-    static constexpr uint32_t kOffBar = kOffSide + kSide * 16 * 4;
+    static constexpr uint32_t kOffLens = kOffSide + kSide * 16 * 4;
+    static constexpr uint32_t kOffBar = kOffLens + kLens * 4;
     static constexpr uint32_t kSmem = 1024 + kOffBar + 512;
     static_assert(kSmem <= 232448, "fits the 227 KB opt-in shared memory");
     static_assert(kSmem > 116 * 1024 || kStages == 10, "one CTA per SM is what the ring is sized for");
@@ -113,7 +116,7 @@ struct Cfg {
 struct AbArgs {
     const void *q, *pk, *pv, *k, *v;   // pk .. v: F32 loaders only
     const int *lens;
-    int *cum;                    // [n_seq + 1] tiles of the sequences before b (one KV head's)
+    int *cum;                    // [n_seq + 1] list places of the sequences before b (one unit each)
     float *part_p, *part_o;      // partial O of prefix and own units
     float2 *ml_p, *ml_o;         // their (m, l)
     float *score;                // add_weights: x_j [n_seq][n_head][pitch]
@@ -130,24 +133,29 @@ struct AbArgs {
 
 __host__ __device__ inline int tiles_of(int rows) { return (rows + kTile - 1) / kTile; }
 
-__device__ __forceinline__ int own_len(const AbArgs &a, int b) {
-    const int n = __ldcg(a.lens + b);
-    return n < 0 || n > a.max_ctx ? 0 : n;
-}
+// List places of a unit over n rows: its tiles after kPad empty ones.
+__host__ __device__ inline int places_of(int rows) { return rows > 0 ? kPad + tiles_of(rows) : 0; }
 
-// The tile list: prefix tiles first, then per sequence its units.  CTA c takes
-// `per` tiles, the first `rem` CTAs one more.  (The host bounds every index.)
+// A length outside the cache counts as 0.
+__device__ __forceinline__ int checked_len(const AbArgs &a, int n) { return n < 0 || n > a.max_ctx ? 0 : n; }
+
+// The list: the prefix units' places first, then per sequence its units'.
+// CTA c takes `per` places, the first `rem` CTAs one more.  A segment's ends
+// (Q, the pipeline's fill and drain, the partial) take as long as about three
+// tiles; without empty places for them, CTAs with many short units finish last
+// (64 sequences of 500 rows behind a prefix of 16384: 69 us, with them see below).
+// (The host bounds every index.)
 struct List {
-    int tp, total;         // prefix tiles, all tiles
-    int lt;                // tiles of a prefix unit
+    int tp, total;         // places of the prefix units, all places
+    int lt;                // places of a prefix unit
     int units_o;           // own units per sequence
     int per, rem;
 
-    __device__ __forceinline__ List(const AbArgs &a, int ndv, int own_tiles) {
-        lt = tiles_of(a.prefix);
+    __device__ __forceinline__ List(const AbArgs &a, int ndv, int own_places) {
+        lt = places_of(a.prefix);
         tp = a.n_kv * a.m_p * ndv * lt;
         units_o = a.n_kv * a.m_o * ndv;
-        total = tp + own_tiles * units_o;
+        total = tp + own_places * units_o;
         per = total / kGrid;
         rem = total - per * kGrid;
     }
@@ -172,47 +180,55 @@ struct Seg {
 struct Walk {
     int t, end;
     int b;
-    int c0;                // list position of sequence b's first own tile, less tp
-    int n, nt;             // length and tiles of sequence b
+    int c0;                // list place of sequence b's first, less tp
+    int n, np;             // length and places of a unit of sequence b
+    const int *lens_s;     // the first kLens lengths
 
     template <int NDV>
     __device__ __forceinline__ bool next(const AbArgs &a, const List &l, Seg &s) {
-        if (t >= end) return false;
-        int u, units;
-        if (t < l.tp) {
-            u = t / l.lt;
-            s.prefix = true;
-            s.j0 = t - u * l.lt;
-            s.j1 = min(l.lt, s.j0 + (min(end, l.tp) - t));
-            s.n = a.prefix;
-            s.slot = blockIdx.x + u;
-            units = a.m_p;
-            s.b = 0;
-        } else {
-            const int o = t - l.tp;
 #pragma unroll 1
-            while (o >= c0 + nt * l.units_o) {
-                c0 += nt * l.units_o;
-                ++b;
-                n = own_len(a, b);
-                nt = tiles_of(n);
+        for (;;) {
+            if (t >= end) return false;
+            int u, units, p0, places;
+            if (t < l.tp) {
+                u = t / l.lt;
+                p0 = t - u * l.lt;
+                places = l.lt;
+                s.prefix = true;
+                s.n = a.prefix;
+                s.slot = blockIdx.x + u;
+                units = a.m_p;
+                s.b = 0;
+            } else {
+                const int o = t - l.tp;
+#pragma unroll 1
+                while (o >= c0 + np * l.units_o) {
+                    c0 += np * l.units_o;
+                    ++b;
+                    n = checked_len(a, b < kLens ? lens_s[b] : __ldcg(a.lens + b));
+                    np = places_of(n);
+                }
+                u = (o - c0) / np;
+                p0 = o - c0 - u * np;
+                places = np;
+                s.prefix = false;
+                s.n = n;
+                s.slot = blockIdx.x + b * l.units_o + u;
+                units = a.m_o;
+                s.b = b;
             }
-            u = (o - c0) / nt;
-            s.prefix = false;
-            s.j0 = o - c0 - u * nt;
-            s.j1 = min(nt, s.j0 + (end - t));
-            s.n = n;
-            s.slot = blockIdx.x + b * l.units_o + u;
-            units = a.m_o;
-            s.b = b;
+            const int p1 = min(places, p0 + (end - t));
+            t += p1 - p0;
+            s.j0 = max(0, p0 - kPad);
+            s.j1 = p1 - kPad;
+            if (s.j1 <= s.j0) continue;      // empty places only
+            const int v = u / NDV;
+            s.dv = u - v * NDV;
+            s.g = units == 1 ? v : v / units;
+            s.m = v - s.g * units;
+            s.rows = min(kM, (s.prefix ? a.n_seq * a.group : a.group) - s.m * kM);
+            return true;
         }
-        const int v = u / NDV;
-        s.dv = u - v * NDV;
-        s.g = units == 1 ? v : v / units;
-        s.m = v - s.g * units;
-        s.rows = min(kM, (s.prefix ? a.n_seq * a.group : a.group) - s.m * kM);
-        t += s.j1 - s.j0;
-        return true;
     }
 };
 
@@ -438,14 +454,12 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     }
     pdl_wait();
     // ---- the list: its length, and where this CTA's own tiles begin ---------------------
-    // the lengths, one read for all of them (the softmax warps' scratch holds them)
-    int *lens_s = reinterpret_cast<int *>(smem + C::kOffScratch);
-    constexpr int kHeld = C::kSoftWarps * 4096 / 4;
-    for (int b = threadIdx.x; b < a.n_seq && b < kHeld; b += C::kThreads) lens_s[b] = __ldcg(a.lens + b);
+    // the lengths, one read for all of them
+    int *lens_s = reinterpret_cast<int *>(smem + C::kOffLens);
+    for (int b = threadIdx.x; b < a.n_seq && b < kLens; b += C::kThreads) lens_s[b] = __ldcg(a.lens + b);
     __syncthreads();
     if (warp == 0) {
-        auto length = [&](int b) { return b >= a.n_seq ? 0 : b < kHeld ? lens_s[b] : __ldcg(a.lens + b); };
-        auto tiles = [&](int n) { return n < 0 || n > a.max_ctx ? 0 : tiles_of(n); };
+        auto length = [&](int b) { return b >= a.n_seq ? 0 : b < kLens ? lens_s[b] : __ldcg(a.lens + b); };
         auto scan = [&](int x) {
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -457,7 +471,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         int sum = 0;
 #pragma unroll 1
         for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-            const int n = length(b0 + lane), nt = tiles(n), incl = scan(nt);
+            const int n = length(b0 + lane), nt = places_of(checked_len(a, n)), incl = scan(nt);
             if (blockIdx.x == 0) {
                 if (n < 0 || n > a.max_ctx) atomicOr(a.status, LALB_STATUS_BAD_POSITION);
                 if (b0 + lane < a.n_seq) a.cum[b0 + lane] = sum + incl - nt;
@@ -474,7 +488,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             int run = 0;
 #pragma unroll 1
             for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-                const int n = length(b0 + lane), nt = tiles(n), incl = scan(nt);
+                const int n = length(b0 + lane), nt = places_of(checked_len(a, n)), incl = scan(nt);
                 const uint32_t past = __ballot_sync(0xffffffffu, run + incl > want);
                 if (past) {
                     const int i = __ffs(past) - 1;
@@ -490,7 +504,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             *start_b = sb;
             start[0] = sum;
             start[1] = before;
-            start[2] = n0 < 0 || n0 > a.max_ctx ? 0 : n0;
+            start[2] = checked_len(a, n0);
         }
     }
     __syncthreads();
@@ -508,7 +522,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     walk.b = *start_b;
     walk.c0 = start[1] * list.units_o;
     walk.n = start[2];
-    walk.nt = tiles_of(walk.n);
+    walk.np = places_of(walk.n);
+    walk.lens_s = lens_s;
     Seg s;
 
     if (warp > C::kSoftWarps + C::kLoadWarps) {
@@ -1128,7 +1143,7 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
     const int g = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_launch_dependents();
-    const int cum = __ldcg(a.cum + b), nt = __ldcg(a.cum + b + 1) - cum;
+    const int cum = __ldcg(a.cum + b), places = __ldcg(a.cum + b + 1) - cum;
     const List l(a, C::kNDV, __ldcg(a.cum + a.n_seq));
     const int n_out = blockIdx.z == 0 ? C::kNDV : 1;    // the weights need one half's sums only
     const bool out = blockIdx.z == 0;
@@ -1139,13 +1154,13 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
         const int up = (g * a.m_p + rp / kM) * C::kNDV + dv, uo = (g * a.m_o + hh / kM) * C::kNDV + dv;
         int np = 0, no = 0, cp = 0, co = 0;
         if (l.lt > 0) {
-            cp = l.owner(up * l.lt);
+            cp = l.owner(up * l.lt + kPad);
             np = l.owner(up * l.lt + l.lt - 1) - cp + 1;
         }
-        if (nt > 0) {
-            const int to = l.tp + cum * l.units_o + uo * nt;
-            co = l.owner(to);
-            no = l.owner(to + nt - 1) - co + 1;
+        if (places > 0) {
+            const int to = l.tp + cum * l.units_o + uo * places;
+            co = l.owner(to + kPad);
+            no = l.owner(to + places - 1) - co + 1;
         }
         const size_t r0p = (size_t)(cp + up) * a.rows_p + rp % kM;
         const size_t r0o = (size_t)(co + b * l.units_o + uo) * a.rows_o + hh % kM;
@@ -1200,7 +1215,7 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
     }
     if (!a.add_weights) return;
     __syncthreads();
-    const int n = own_len(a, b);
+    const int n = checked_len(a, __ldcg(a.lens + b));
     const float *sc = a.score + ((size_t)b * a.n_head + (size_t)g * a.group) * a.pitch;
     float *w = a.row_weight + ((size_t)b * a.n_kv + g) * a.max_ctx;
     for (int j = blockIdx.z * 32 * kCombWarps + threadIdx.x; j < n; j += gridDim.z * 32 * kCombWarps) {
@@ -1225,10 +1240,10 @@ int ab_shape(const lalb_kv_batch *c, const lalb_attn_batch *p) {
     if (group > kMaxGroup || (long long)p->n_head * c->head_dim > (1 << 24) || c->n_seq > 65535 ||
         c->n_kv_head > 65535)
         return LALB_ERR_UNSUPPORTED;
-    // tiles of the list at most, and query rows: 31-bit indices
+    // places of the list at most, and query rows: 31-bit indices
     const long long mp = (c->n_seq * group + kM - 1) / kM, mo = (group + kM - 1) / kM;
-    const long long tiles = 2ll * c->n_kv_head * (mp * tiles_of(p->prefix_len) +
-                                                  mo * c->n_seq * (long long)tiles_of(c->max_ctx));
+    const long long tiles = 2ll * c->n_kv_head * (mp * places_of(p->prefix_len) +
+                                                  mo * c->n_seq * (long long)places_of(c->max_ctx));
     if (tiles > (1ll << 30) || c->n_seq * group > (1ll << 30)) return LALB_ERR_UNSUPPORTED;
     return LALB_OK;
 }
