@@ -63,7 +63,7 @@ constexpr int kLens = 512;           // sequences whose lengths a CTA keeps in s
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (loaders run at most 5 ahead)
 constexpr float kShift = 6.0f;       // weights up to 2^6 at the reference maximum, 2^14 before a rescale
 constexpr float kGrow = 8.0f;        // growth of a row's maximum that is left in place
-constexpr int kStageBudget2 = 160 * 1024, kStageBudget1 = 192 * 1024;
+constexpr int kStageBudget2 = 160 * 1024, kStageBudget1 = 192 * 1024, kStageBudgetRaw = 128 * 1024;
 
 template <class T, int HD>
 struct Cfg {
@@ -97,14 +97,19 @@ struct Cfg {
                                         kEven * (kSoftWarps + kOtherWarps),
                   "the split is no more than the block was launched with");
     static constexpr uint32_t kStage = kTile * HD * (kF32 ? 4 : 2);
-    static constexpr int kBudget = kNS == 2 ? kStageBudget2 : kStageBudget1;
+    // F32 rows come in raw, 8 of them at a time into one of two slots of the
+    // loader warp that splits them (head_dim 256 has no room: plain loads)
+    static constexpr bool kRaw = kF32 && kDV == HD;
+    static constexpr uint32_t kGroup = 8 * HD * 4;
+    static constexpr int kBudget = kRaw ? kStageBudgetRaw : kNS == 2 ? kStageBudget2 : kStageBudget1;
     static constexpr int kStages = kBudget / (int)kStage < 10 ? kBudget / (int)kStage : 10;
     static_assert(kStages >= 2 * kAhead + 1, "V(j) to K(j + kAhead) are held at once");
     static_assert(kStages / 2 + 2 <= kSide, "a tile's scales outlive its stages");
     static constexpr int kSubW = HD < 64 ? HD : 64;                   // columns of a swizzled subtile
     static constexpr uint32_t kSub = kTile * kSubW * 2;               // its bytes
     static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
-    static constexpr uint32_t kOffMl = kOffScratch + kSoftWarps * 4096;
+    static constexpr uint32_t kOffRaw = kOffScratch + kSoftWarps * 4096;
+    static constexpr uint32_t kOffMl = kOffRaw + (kRaw ? kLoadWarps * 2 * kGroup : 0);
     static constexpr uint32_t kOffSide = kOffMl + 2 * (2 * kM * 8 + 32);   // ml and qmax, of two segments
     static constexpr uint32_t kOffLens = kOffSide + kSide * 16 * 4;
     static constexpr uint32_t kOffBar = kOffLens + kLens * 4;
@@ -383,12 +388,24 @@ struct RowLoad {
                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
     }
+    // The same from the 8 rows as they lie in shared memory.
+    __device__ __forceinline__ void load_raw(const uint8_t *raw, int left, int lane) {
+        const int rr = lane / kLanes, cc = (lane % kLanes) * 4;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int r = i / kVec * kPer + rr, c = cc + (i % kVec) * 4 * kLanes;
+            x[i] = r < left ? *reinterpret_cast<const float4 *>(raw + r * (COLS * 4) + c * 4)
+                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
     // The rows' common exponent.
     __device__ __forceinline__ int exponent() const {
-        float m = 0.0f;
+        float m4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kN; ++i)
-            m = fmaxf(m, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+            m4[i & 3] = fmaxf(m4[i & 3],
+                              fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         return part_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
     }
     __device__ __forceinline__ void store(uint8_t *stage, int r0, float scale, int lane) const {
@@ -427,6 +444,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     uint64_t *qready = ofull + 2;              // Q of the segment written
     uint64_t *oready = qready + 1;             // O of the segment read
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(oready + 1);
+    uint64_t *rawfull = reinterpret_cast<uint64_t *>(smem + C::kOffBar + 384);    // [loader warp][slot]
     int *start_b = reinterpret_cast<int *>(tmem_slot + 1);
     int *start = start_b + 1;                  // own tiles of all, of those before start_b, start_b's length
 
@@ -441,6 +459,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             mbar_init(&pready[s], 4);
         }
         for (int s = 0; s < 2; ++s) mbar_init(&ofull[s], 1);
+        if constexpr (C::kRaw)
+            for (int k = 0; k < 2 * C::kLoadWarps; ++k) mbar_init(&rawfull[k], 1);
         mbar_init(qready, C::kSoftWarps);
         mbar_init(oready, C::kSoftWarps);
         fence_barrier_init();
@@ -540,8 +560,10 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             const float *kb = nullptr, *vb = nullptr;
             bool ok = true;
             struct Task {
-                const float *p;
-                int left, k;
+                const float *p;      // plain loads: the rows
+                int left, k;         // rows of the cache from the first one on; the group's number
+                int row;             // raw: the first row in its tensor map
+                bool prefix;
             };
             auto advance = [&](Task &t) -> bool {
                 const int tile = k >> 4;
@@ -557,6 +579,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 const int row = (s.j0 + tile - t0) * kTile + 8 * (k & 7);
                 t.p = ((k >> 3) & 1 ? vb : kb) + (size_t)row * pitch;
                 t.left = s.n - row;
+                t.row = row + (s.prefix ? 0 : s.b * a.max_ctx);
+                t.prefix = s.prefix;
                 t.k = k;
                 k += C::kLoadWarps;
                 return true;
@@ -573,21 +597,45 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 if (lane == 0) mbar_arrive(&full[slot]);
             };
             Task t;
-            if constexpr (C::kDV == HD) {
-                // the next group's loads are in flight while this one is converted
-                RowLoad<HD> x;
-                bool more = advance(t);
-                if (more) x.load(t.p, pitch, t.left, lane);
+            if constexpr (C::kRaw) {
+                // two groups on their way: a third starts into a slot as soon as the
+                // warp has its rows in registers
+                const int w = warp - C::kSoftWarps - 1;
+                uint8_t *raw = smem + C::kOffRaw + w * 2 * C::kGroup;
+                uint64_t *bar = rawfull + 2 * w;
+                auto issue = [&](const Task &u, int slot) {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&bar[slot], C::kGroup);
+                        const bool v = (u.k >> 3) & 1;
+                        const CUtensorMap *m = u.prefix ? (v ? &mPV : &mPK) : (v ? &mV : &mK);
+                        tma2d(raw + slot * C::kGroup, m, s.g * HD, u.row, &bar[slot]);
+                    }
+                };
+                Task q0, q1;
+                int issued = 0, taken = 0;
+                if (advance(q0)) issue(q0, 0), ++issued;
+                if (issued && advance(q1)) issue(q1, 1), ++issued;
 #pragma unroll 1
-                while (more && ok) {
-                    Task u;
-                    RowLoad<HD> y;
-                    more = advance(u);
-                    if (more) y.load(u.p, pitch, u.left, lane);
-                    finish(x, t.k);
-                    x = y;
-                    t = u;
+                while (taken < issued && ok) {
+                    const int slot = taken & 1;
+                    const int left = slot ? q1.left : q0.left, kk = slot ? q1.k : q0.k;
+                    ok = warp_wait(&bar[slot], (taken >> 1) & 1u, a.status);
+                    RowLoad<HD> x;
+                    x.load_raw(raw + slot * C::kGroup, left, lane);
+                    ++taken;
+                    __syncwarp();
+                    if (issued == taken + 1 && advance(t)) {
+                        issue(t, slot);
+                        ++issued;
+                        if (slot)
+                            q1 = t;
+                        else
+                            q0 = t;
+                    }
+                    finish(x, kk);
                 }
+                // nothing may still be on its way into this CTA's shared memory when it ends
+                for (; taken < issued; ++taken) (void)warp_wait(&bar[taken & 1], (taken >> 1) & 1u, a.status);
             } else {
 #pragma unroll 1
                 while (ok && advance(t)) {
@@ -1376,16 +1424,21 @@ extern "C" int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache, c
                                                      : kernels_for<__nv_bfloat16>(a.hd);
     if (int st = lalb_set_smem_attr(ctx, kn.tiles, kn.smem)) return st;
     CUtensorMap maps[4] = {};
-    if (es == 2) {
-        const CUtensorMapDataType dt =
-            cache->dtype == LALB_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        const int box = std::min(64, a.hd);
-        const CUtensorMapSwizzle sw = box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    {
+        // 16 bits: swizzled 64-column tiles of 64 rows; F32: 8 plain rows of a head
+        const CUtensorMapDataType dt = es == 4                         ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : cache->dtype == LALB_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        const int box = es == 4 ? a.hd : std::min(64, a.hd), rows_box = es == 4 ? 8 : kTile;
+        const CUtensorMapSwizzle sw = es == 4     ? CU_TENSOR_MAP_SWIZZLE_NONE
+                                      : box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                                  : CU_TENSOR_MAP_SWIZZLE_64B;
         const void *base[4] = {a.pk, a.pv, a.k, a.v};
         for (int i = 0; i < 4; ++i) {
             const long long rows = i < 2 ? a.prefix : (long long)a.n_seq * a.max_ctx;
             if (rows == 0) continue;
-            if (int st = map2d(ctx, &maps[i], base[i], dt, 2, (long long)a.n_kv * a.hd, rows, box, kTile, sw)) return st;
+            if (int st = map2d(ctx, &maps[i], base[i], dt, es, (long long)a.n_kv * a.hd, rows, box, rows_box, sw))
+                return st;
         }
     }
     if (int st = launch_pdl(ctx, kn.tiles, dim3(kGrid), dim3(kn.threads), kn.smem, (cudaStream_t)stream,
