@@ -33,8 +33,8 @@
 //            = TMEM lanes = threads, so rows need no shuffles); O is rescaled
 //            only when a row's maximum has grown by more than 2^8.
 //
-// F32: x = hi + lo in fp16 (22 bits), three of the four products.  The eight
-// rows of a tile that a loader warp converts share a power of two that puts
+// F32: x = hi + lo in fp16 (22 bits), three of the four products.  The rows of
+// a tile that a loader warp splits at a time share a power of two that puts
 // their largest |x| in [2^14, 2^15); K's goes into the scores' factor, V's
 // exponent e into the weights' exponent: p' = 2^(x + e - m), v' = v 2^-e, so
 // that p' keeps its precision whatever the values' range, and l takes
@@ -85,7 +85,9 @@ struct Cfg {
     static constexpr int kSoftWarps = 4 * kNS;
     // F32: 7, which with the MMA warp makes two warpgroups
     static constexpr int kLoadWarps = kF32 ? 7 : 1;
-    static constexpr int kFullCount = kF32 ? 8 : 1;    // arrivals that fill a stage: its groups of 8 rows
+    // F32: rows that a loader warp splits at a time, under one power of two
+    static constexpr int kRows = HD == 256 ? 8 : 16, kGroups = kTile / kRows;
+    static constexpr int kFullCount = kF32 ? kGroups : 1;    // arrivals that fill a stage
     static constexpr int kOtherWarps = kF32 ? 8 : 4;   // MMA, loaders (16 bits: two warps idle)
     static constexpr int kThreads = 32 * (kSoftWarps + kOtherWarps);
     // Registers a thread: the launch's even share, and the split of it (the
@@ -97,10 +99,11 @@ struct Cfg {
                                         kEven * (kSoftWarps + kOtherWarps),
                   "the split is no more than the block was launched with");
     static constexpr uint32_t kStage = kTile * HD * (kF32 ? 4 : 2);
-    // F32 rows come in raw, 8 of them at a time into one of two slots of the
-    // loader warp that splits them (head_dim 256 has no room: plain loads)
+    // F32 rows come in raw, a group at a time, into a slot of the loader warp
+    // that splits them (head_dim 256 has no room: plain loads)
     static constexpr bool kRaw = kF32 && kDV == HD;
-    static constexpr uint32_t kGroup = 8 * HD * 4;
+    static constexpr uint32_t kGroup = kRows * HD * 4;
+    static constexpr int kSlots = HD == 128 ? 1 : 2;
     static constexpr int kBudget = kRaw ? kStageBudgetRaw : kNS == 2 ? kStageBudget2 : kStageBudget1;
     static constexpr int kStages = kBudget / (int)kStage < 10 ? kBudget / (int)kStage : 10;
     static_assert(kStages >= 2 * kAhead + 1, "V(j) to K(j + kAhead) are held at once");
@@ -109,7 +112,7 @@ struct Cfg {
     static constexpr uint32_t kSub = kTile * kSubW * 2;               // its bytes
     static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
     static constexpr uint32_t kOffRaw = kOffScratch + kSoftWarps * 4096;
-    static constexpr uint32_t kOffMl = kOffRaw + (kRaw ? kLoadWarps * 2 * kGroup : 0);
+    static constexpr uint32_t kOffMl = kOffRaw + (kRaw ? kLoadWarps * kSlots * kGroup : 0);
     static constexpr uint32_t kOffSide = kOffMl + 2 * (2 * kM * 8 + 32);   // ml and qmax, of two segments
     static constexpr uint32_t kOffLens = kOffSide + kSide * 16 * 4;
     static constexpr uint32_t kOffBar = kOffLens + kLens * 4;
@@ -368,15 +371,15 @@ constexpr uint32_t mma_idesc(int n, bool b_mn) {
            ((uint32_t)(kM >> 4) << 24);
 }
 
-// ---- F32 loaders: eight rows of a tile by one warp -------------------------------------
-// Rows r0 .. r0 + 7 of the tile (cache rows row0 + r0 ..; rows at or past n
-// are zeros), COLS columns from src: registers first, then split and stored.
-template <int COLS>
+// ---- F32 loaders: a group of ROWS rows of a tile by one warp ----------------------------
+// COLS columns of each (rows at or past the end are zeros): registers first,
+// then split and stored.
+template <int COLS, int ROWS>
 struct RowLoad {
     static constexpr int kLanes = COLS / 4 < 32 ? COLS / 4 : 32;   // lanes of one row
     static constexpr int kPer = 32 / kLanes;                       // rows per load
     static constexpr int kVec = COLS / (4 * kLanes);               // loads of one row
-    static constexpr int kN = 8 / kPer * kVec;
+    static constexpr int kN = ROWS / kPer * kVec;
     float4 x[kN];
 
     __device__ __forceinline__ void load(const float *src, size_t pitch, int left, int lane) {
@@ -388,7 +391,7 @@ struct RowLoad {
                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
     }
-    // The same from the 8 rows as they lie in shared memory.
+    // The same from the rows as they lie in shared memory.
     __device__ __forceinline__ void load_raw(const uint8_t *raw, int left, int lane) {
         const int rr = lane / kLanes, cc = (lane % kLanes) * 4;
 #pragma unroll
@@ -460,7 +463,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         }
         for (int s = 0; s < 2; ++s) mbar_init(&ofull[s], 1);
         if constexpr (C::kRaw)
-            for (int k = 0; k < 2 * C::kLoadWarps; ++k) mbar_init(&rawfull[k], 1);
+            for (int k = 0; k < C::kSlots * C::kLoadWarps; ++k) mbar_init(&rawfull[k], 1);
         mbar_init(qready, C::kSoftWarps);
         mbar_init(oready, C::kSoftWarps);
         fence_barrier_init();
@@ -552,7 +555,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         set_regs<C::kSoftRegs ? C::kOtherRegs : 0, false>();
         // ================================ loaders ===============================================
         if constexpr (C::kF32) {
-            // A stage is 8 groups of 8 rows; the groups go round the loader warps:
+            // A stage is kGroups groups of rows, which go round the loader warps:
             // warp w has groups w, w + 7, w + 14, .. of the CTA's stages.
             const size_t pitch = (size_t)a.n_kv * HD;
             int k = warp - C::kSoftWarps - 1;            // the next group to look at
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 bool prefix;
             };
             auto advance = [&](Task &t) -> bool {
-                const int tile = k >> 4;
+                const int tile = k / (2 * C::kGroups);
 #pragma unroll 1
                 while (tile >= t1) {
                     if (!walk.template next<C::kNDV>(a, list, s)) return false;
@@ -576,8 +579,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     kb = static_cast<const float *>(s.prefix ? a.pk : a.k) + seq + (size_t)s.g * HD;
                     vb = static_cast<const float *>(s.prefix ? a.pv : a.v) + seq + (size_t)s.g * HD + s.dv * C::kDV;
                 }
-                const int row = (s.j0 + tile - t0) * kTile + 8 * (k & 7);
-                t.p = ((k >> 3) & 1 ? vb : kb) + (size_t)row * pitch;
+                const int row = (s.j0 + tile - t0) * kTile + C::kRows * (k % C::kGroups);
+                t.p = (k / C::kGroups & 1 ? vb : kb) + (size_t)row * pitch;
                 t.left = s.n - row;
                 t.row = row + (s.prefix ? 0 : s.b * a.max_ctx);
                 t.prefix = s.prefix;
@@ -586,10 +589,10 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 return true;
             };
             auto finish = [&](const auto &x, int k) {
-                const uint32_t st = k >> 3, g = k & 7, slot = st % C::kStages, use = st / C::kStages;
+                const uint32_t st = k / C::kGroups, g = k % C::kGroups, slot = st % C::kStages, use = st / C::kStages;
                 const int e = x.exponent();
                 if (use > 0) ok = ok && warp_wait(&empty[slot], (use - 1) & 1u, a.status);
-                x.store(smem + slot * C::kStage, 8 * g, pow2(-e), lane);
+                x.store(smem + slot * C::kStage, C::kRows * g, pow2(-e), lane);
                 // K: the factor that undoes the scaling; V: the exponent
                 if (lane == 0) side[((st >> 1) % kSide) * 16 + (st & 1) * 8 + g] = st & 1 ? (float)e : pow2(e);
                 fence_async();
@@ -598,15 +601,15 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             };
             Task t;
             if constexpr (C::kRaw) {
-                // two groups on their way: a third starts into a slot as soon as the
+                // kSlots groups on their way: the next starts into a slot as soon as the
                 // warp has its rows in registers
                 const int w = warp - C::kSoftWarps - 1;
-                uint8_t *raw = smem + C::kOffRaw + w * 2 * C::kGroup;
-                uint64_t *bar = rawfull + 2 * w;
+                uint8_t *raw = smem + C::kOffRaw + w * C::kSlots * C::kGroup;
+                uint64_t *bar = rawfull + C::kSlots * w;
                 auto issue = [&](const Task &u, int slot) {
                     if (lane == 0) {
                         mbar_arrive_expect_tx(&bar[slot], C::kGroup);
-                        const bool v = (u.k >> 3) & 1;
+                        const bool v = u.k / C::kGroups & 1;
                         const CUtensorMap *m = u.prefix ? (v ? &mPV : &mPK) : (v ? &mV : &mK);
                         tma2d(raw + slot * C::kGroup, m, s.g * HD, u.row, &bar[slot]);
                     }
@@ -614,17 +617,17 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 Task q0, q1;
                 int issued = 0, taken = 0;
                 if (advance(q0)) issue(q0, 0), ++issued;
-                if (issued && advance(q1)) issue(q1, 1), ++issued;
+                if (C::kSlots == 2 && issued && advance(q1)) issue(q1, 1), ++issued;
 #pragma unroll 1
                 while (taken < issued && ok) {
-                    const int slot = taken & 1;
+                    const int slot = taken % C::kSlots;
                     const int left = slot ? q1.left : q0.left, kk = slot ? q1.k : q0.k;
-                    ok = warp_wait(&bar[slot], (taken >> 1) & 1u, a.status);
-                    RowLoad<HD> x;
+                    ok = warp_wait(&bar[slot], (taken / C::kSlots) & 1u, a.status);
+                    RowLoad<HD, C::kRows> x;
                     x.load_raw(raw + slot * C::kGroup, left, lane);
                     ++taken;
                     __syncwarp();
-                    if (issued == taken + 1 && advance(t)) {
+                    if (issued == taken + C::kSlots - 1 && advance(t)) {
                         issue(t, slot);
                         ++issued;
                         if (slot)
@@ -635,16 +638,16 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     finish(x, kk);
                 }
                 // nothing may still be on its way into this CTA's shared memory when it ends
-                for (; taken < issued; ++taken) (void)warp_wait(&bar[taken & 1], (taken >> 1) & 1u, a.status);
+                for (; taken < issued; ++taken) (void)warp_wait(&bar[taken % C::kSlots], (taken / C::kSlots) & 1u, a.status);
             } else {
 #pragma unroll 1
                 while (ok && advance(t)) {
-                    if ((t.k >> 3) & 1) {
-                        RowLoad<C::kDV> x;
+                    if (t.k / C::kGroups & 1) {
+                        RowLoad<C::kDV, C::kRows> x;
                         x.load(t.p, pitch, t.left, lane);
                         finish(x, t.k);
                     } else {
-                        RowLoad<HD> x;
+                        RowLoad<HD, C::kRows> x;
                         x.load(t.p, pitch, t.left, lane);
                         finish(x, t.k);
                     }
@@ -1026,7 +1029,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         const uint32_t sc = lanes + C::kColS + buf * kTile;
                         const float *sd = side + (t % kSide) * 16;
                         // never 0: -inf (a row past the end) times it has to stay -inf
-                        auto factor = [&](int g) { return fmaxf(sd[g] * cq, 1e-37f); };
+                        auto factor = [&](int g) { return fmaxf(sd[8 * g / C::kRows] * cq, 1e-37f); };   // of columns 8 g ..
+                        auto exponent = [&](int g) { return sd[8 + 8 * g / C::kRows]; };
                         auto past_end = [&](float *y, int j0, int nj) {
                             if (valid < kTile) {
 #pragma unroll
@@ -1064,7 +1068,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                                 past_end(y, 32 * h, 32);
 #pragma unroll
                                 for (int g = 0; g < 4; ++g) {
-                                    const float f = factor(4 * h + g), e = sd[8 + 4 * h + g];
+                                    const float f = factor(4 * h + g), e = exponent(4 * h + g);
 #pragma unroll
                                     for (int j = 0; j < 8; j += 2) {
                                         const float2 v = __ffma2_rn(make_float2(y[8 * g + j], y[8 * g + j + 1]),
@@ -1124,7 +1128,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                                 past_end(y, 16 * kk, 16);
 #pragma unroll
                                 for (int g = 0; g < 2; ++g) {
-                                    const float ev = sd[8 + 2 * kk + g];
+                                    const float ev = exponent(2 * kk + g);
                                     sum2 = make_float2(0.0f, 0.0f);
                                     weigh8(y + 8 * g, factor(2 * kk + g), ev - mref, w + 4 * g, w + 8 + 4 * g);
                                     l = fmaf(sum2.x + sum2.y, pow2(-(int)ev), l);
@@ -1339,14 +1343,14 @@ void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
 
 struct Kernels {
     const void *tiles, *combine;
-    int threads, smem;
+    int threads, smem, rows;
 };
 
 template <class T, int HD>
 Kernels kernels_of() {
     using C = Cfg<T, HD>;
     return {(const void *)attention_tiles_kernel<T, HD>, (const void *)attention_combine_kernel<T, HD>, C::kThreads,
-            (int)C::kSmem};
+            (int)C::kSmem, C::kRows};
 }
 
 template <class T>
@@ -1425,11 +1429,11 @@ extern "C" int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache, c
     if (int st = lalb_set_smem_attr(ctx, kn.tiles, kn.smem)) return st;
     CUtensorMap maps[4] = {};
     {
-        // 16 bits: swizzled 64-column tiles of 64 rows; F32: 8 plain rows of a head
+        // 16 bits: swizzled 64-column tiles of 64 rows; F32: a loader warp's plain rows of a head
         const CUtensorMapDataType dt = es == 4                         ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                        : cache->dtype == LALB_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        const int box = es == 4 ? a.hd : std::min(64, a.hd), rows_box = es == 4 ? 8 : kTile;
+        const int box = es == 4 ? a.hd : std::min(64, a.hd), rows_box = es == 4 ? kn.rows : kTile;
         const CUtensorMapSwizzle sw = es == 4     ? CU_TENSOR_MAP_SWIZZLE_NONE
                                       : box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B
                                                   : CU_TENSOR_MAP_SWIZZLE_64B;
