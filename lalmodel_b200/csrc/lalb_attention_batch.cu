@@ -16,6 +16,13 @@
 // time; an own unit fills only its group's lanes of the M = 128 instructions,
 // which costs tensor time that a memory-bound unit has to spare.
 //
+// Units of at most 16 rows (few sequences, and the own units of all common head
+// layouts) leave three of four softmax warps without a row.  Where the softmax
+// is what such a unit waits for (Cfg::kFewOk), its Q is written four times, once
+// to each warp's 32 lanes, and warp w takes only scores 16 w .. 16 w + 15 of a
+// tile, with zeros as the weights of the rest; the four warps' sums are added
+// at the segment's end.
+//
 // Split.  All tiles of all units form one list, and CTA c of G (one per SM)
 // takes tiles [c W / G, (c + 1) W / G): equal shares whatever the lengths,
 // without the host knowing them.  A run of tiles of one unit in one CTA (a
@@ -58,6 +65,7 @@ namespace {
 constexpr int kGrid = 148;           // one CTA per SM of a B200 (workspace sizes need no device)
 constexpr int kTile = 64;            // cache rows per tile
 constexpr int kM = 128;              // query rows per unit
+constexpr int kFew = 16;             // units of at most so many rows: a tile's columns are split over the warps
 constexpr int kPad = 3;              // list places a unit takes beside its tiles: what its segment's ends cost
 constexpr int kLens = 512;           // sequences whose lengths a CTA keeps in shared memory
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (loaders run at most 5 ahead)
@@ -108,6 +116,12 @@ struct Cfg {
     static constexpr int kStages = kBudget / (int)kStage < 10 ? kBudget / (int)kStage : 10;
     static_assert(kStages >= 2 * kAhead + 1, "V(j) to K(j + kAhead) are held at once");
     static_assert(kStages / 2 + 2 <= kSide, "a tile's scales outlive its stages");
+    // Narrow heads' tiles come in faster than one warp weighs them (8 sequences
+    // of 3001 to 8191 scored f16 rows at head_dim 64: 45 us without, 39 with; F32
+    // 70 and 69); wide ones wait for memory or the loaders, and four Qs and the
+    // sum at the end cost more than they give (64 sequences of up to 1000 bf16
+    // rows behind a prefix, head_dim 128: 69 and 77; one of 64 F32 rows 17 and 18)
+    static constexpr bool kFewOk = HD <= 64;
     static constexpr int kSubW = HD < 64 ? HD : 64;                   // columns of a swizzled subtile
     static constexpr uint32_t kSub = kTile * kSubW * 2;               // its bytes
     static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
@@ -134,7 +148,7 @@ struct AbArgs {
     long long q_stride;
     int n_seq, n_head, n_kv, group, hd, max_ctx, prefix, add_weights;
     int m_p, m_o;                // 128-row tiles of a prefix and an own unit's KV head
-    int rows_p, rows_o;          // rows kept per partial
+    int rows_p, rows_o;          // rows kept per partial: query rows of a prefix and an own unit at most
     int pitch;
     float c, decay, sign;        // |scale| log2 e, sign of the scale
 };
@@ -771,6 +785,12 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         uint32_t tile = 0;                      // before the segment
         uint32_t pv0 = 0, pv1 = 0;              // products of each stream so far
         bool ok = true;
+        auto wg_bar = [&]() {      // one warpgroup
+            if (C::kNS == 2 && wg)
+                asm volatile("bar.sync 3, 128;" ::: "memory");
+            else
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+        };
         auto soft_bar = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kSoftWarps) : "memory"); };
 
         // ---- Q: this warp's 32 rows, the 32-column chunks of its warpgroup, into TMEM ----------------
@@ -781,10 +801,12 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         const bool q_idle = wg >= HD / 32;      // head_dim 32: one chunk, the first warpgroup's
         constexpr int kBatch = 16 / kIt < kChunks ? 16 / kIt : kChunks;         // chunks per batch
         const int lr = lane / kLpr, lu = lane % kLpr;
+        auto few = [&](const Seg &g) { return C::kFewOk && (g.prefix ? a.rows_p : a.rows_o) <= kFew; };
+        auto first_row = [&](const Seg &g) { return few(g) ? 0 : quarter * 32; };   // the warp's first row
         auto q_load = [&](const Seg &g, int c0, uint4 (&v)[kBatch * kIt]) {
             const T *qb = static_cast<const T *>(a.q) + (size_t)g.g * a.group * HD + (c0 * C::kNS + wg) * 32;
             // row r of the unit: head h of sequence b, and kRpi rows further each time
-            int r = quarter * 32 + lr, b = g.b, h = g.m * kM + r;
+            int r = first_row(g) + lr, b = g.b, h = g.m * kM + r;
             if (g.prefix) {
                 b = h / a.group;
                 h -= b * a.group;
@@ -844,12 +866,12 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         uint4 qv[kBatch * kIt];
         // before the barrier both warpgroups pass at a segment's start ..
         auto q_begin = [&](const Seg &g) {
-            if (quarter * 32 >= g.rows || q_idle) return;
+            if (first_row(g) >= g.rows || q_idle) return;
             q_load(g, 0, qv);
         };
         auto q_share = [&](const Seg &g) {
             if constexpr (C::kF32) {
-                if (quarter * 32 >= g.rows || q_idle) return;
+                if (first_row(g) >= g.rows || q_idle) return;
                 float top = q_top(qv, 0.0f);
 #pragma unroll 1
                 for (int c = kBatch; c < kChunks; c += kBatch) {
@@ -865,7 +887,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         // rows' score factor returned
         auto q_finish = [&](const Seg &g) -> float {
             float qs = a.sign, cq = a.c;
-            if (quarter * 32 < g.rows) {
+            if (first_row(g) < g.rows) {
                 if constexpr (C::kF32) {
                     const float *qm = qmax + turn * 8 + quarter;
                     const float top = C::kNS == 2 && HD > 32 ? fmaxf(qm[0], qm[4]) : qm[0];
@@ -892,6 +914,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         int n = 0;                               // the segment's tiles
         bool have = false, had = false;          // a segment is open; one of its tiles was this warpgroup's
         bool active = false;                     // a row of this warp belongs to its unit
+        bool split = false;                      // at most 16 rows: this warp has 16 columns of a tile
+        bool any = false;                        // this thread's row has met a score
         float cq = 0.0f, mref = 0.0f, l = 0.0f;
 #pragma unroll 1
         for (;;) {
@@ -906,29 +930,39 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 const uint32_t k = C::kNS == 2 ? wg : 0;
                 ok = ok && warp_wait(&ofull[k], ((k ? pv1 : pv0) - 1) & 1u, a.status);
             }
-            ml[turn * 2 * kM + wg * kM + row] = make_float2(mref, l);
+            ml[turn * 2 * kM + wg * kM + row] = make_float2(had && any ? mref : -INFINITY, l);
             if (nhave) q_share(nx);
             tc_before();
             soft_bar();
             tc_after();
             const float2 *mlt = ml + turn * 2 * kM;
-            const float2 r0 = mlt[row], r1 = C::kNS == 2 ? mlt[kM + row] : make_float2(0.0f, 0.0f);
+            const float2 r0 = mlt[row], r1 = C::kNS == 2 ? mlt[kM + row] : make_float2(-INFINITY, 0.0f);
             float cn = 0.0f;
             if (nhave) cn = q_finish(nx);
             turn ^= 1;
             if (have) {
-                // a stream without a tile in this segment has nothing (the other has)
-                const bool has0 = C::kNS == 1 || n > 1 || (tile & 1u) == 0, has1 = C::kNS == 2 && (n > 1 || (tile & 1u) == 1);
-                const float m = has0 && has1 ? fmaxf(r0.x, r1.x) : has0 ? r0.x : r1.x;
+                // a stream without a tile in this segment, or a score in this row, has nothing
+                const bool has0 = r0.x > -INFINITY, has1 = r1.x > -INFINITY;
+                float m = fmaxf(r0.x, r1.x), lsum = 0.0f;
+                if (split) {       // the row's sums are in four warps
+#pragma unroll
+                    for (int k = 0; k < 4 * C::kNS; ++k) m = fmaxf(m, mlt[32 * k + lane].x);
+#pragma unroll
+                    for (int k = 0; k < 4 * C::kNS; ++k) {
+                        const float2 x = mlt[32 * k + lane];
+                        lsum = fmaf(x.y, x.x > -INFINITY ? ex2(x.x - m) : 0.0f, lsum);
+                    }
+                }
                 const float f0 = has0 ? ex2(r0.x - m) : 0.0f, f1 = has1 ? ex2(r1.x - m) : 0.0f;
-                if (active && ok) {
+                if (active && (ok || split)) {     // split: all four warps meet at the barriers below
                     const int rows = s.prefix ? a.rows_p : a.rows_o;
-                    const size_t first = (size_t)s.slot * rows + quarter * 32;
+                    const size_t first = (size_t)s.slot * rows + first_row(s);
                     float *po = (s.prefix ? a.part_p : a.part_o) + first * C::kDV;
                     float2 *pm = (s.prefix ? a.ml_p : a.ml_o) + first;
-                    const int live = min(32, s.rows - quarter * 32);
-                    if (wg == 0 && row < s.rows)
-                        pm[lane] = make_float2(m, (has0 ? r0.y * f0 : 0.0f) + (has1 ? r1.y * f1 : 0.0f));
+                    const int live = min(32, s.rows - first_row(s));
+                    if (wg == 0 && lane < live && (!split || quarter == 0))
+                        pm[lane] = make_float2(
+                            m, split ? lsum : (has0 ? r0.y * f0 : 0.0f) + (has1 ? r1.y * f1 : 0.0f));
                     constexpr int kHalf = C::kDV / C::kNS, kP = 16;
                     constexpr int kOl = kP / 4, kOr = 32 / kOl;      // lanes of a row's piece, rows per store
                     const int olr = lane / kOl, olu = lane % kOl;
@@ -942,6 +976,34 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         for (int k = 0; k < kP; ++k) {
                             o[k] = has0 ? o[k] * f0 : 0.0f;
                             if (C::kNS == 2 && has1) o[k] = fmaf(v[k], f1, o[k]);
+                        }
+                        if (split) {
+                            // 64 columns of the warpgroup's at a time: each warp's rows side by
+                            // side, then every thread adds the four warps' for its columns
+                            constexpr int kW = kHalf < 64 ? kHalf : 64;
+                            if (lane < live) {
+#pragma unroll
+                                for (int u = 0; u < kOl; ++u)
+                                    *reinterpret_cast<float4 *>(scratch + lane * kW * 4 +
+                                                                (((c % kW) / 4 + u) ^ (lane & (kW / 4 - 1))) * 16) =
+                                        make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                            }
+                            if ((c + kP) % kW) continue;
+                            wg_bar();
+                            const uint8_t *four = smem + C::kOffScratch + wg * 4 * 4096;
+                            for (int i = quarter * 32 + lane; i < live * (kW / 4); i += 128) {
+                                const int r = i / (kW / 4), u = i % (kW / 4);
+                                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                                for (int w = 0; w < 4; ++w) {
+                                    const float4 v = *reinterpret_cast<const float4 *>(
+                                        four + w * 4096 + r * kW * 4 + (u ^ (r & (kW / 4 - 1))) * 16);
+                                    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+                                }
+                                *reinterpret_cast<float4 *>(po + (size_t)r * C::kDV + (c + kP - kW) + 4 * u) = sum;
+                            }
+                            wg_bar();
+                            continue;
                         }
                         if (live <= 8) {      // a few rows: each lane its own
                             if (lane < live) {
@@ -977,13 +1039,15 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             have = true;
             cq = cn;
             n = s.j1 - s.j0;
-            active = quarter * 32 < s.rows;
+            split = few(s);
+            active = first_row(s) < s.rows;
             mref = l = 0.0f;
-            bool any = false;
+            any = false;
             had = false;
             float *score = nullptr;
-            if (a.add_weights && !s.prefix && s.dv == 0 && row < s.rows)
-                score = a.score + ((size_t)s.b * a.n_head + (size_t)s.g * a.group + s.m * kM + row) * a.pitch;
+            if (a.add_weights && !s.prefix && s.dv == 0 && first_row(s) + lane < s.rows)
+                score = a.score +
+                        ((size_t)s.b * a.n_head + (size_t)s.g * a.group + s.m * kM + first_row(s) + lane) * a.pitch;
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
                 const uint32_t t = tile + i, buf = t % C::kBufs;
@@ -1044,7 +1108,28 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         // code is fetched more slowly than the scores are read.
                         constexpr int kHeld = C::kF32 ? 1 : kTile;
                         float x[kHeld];
-                        if constexpr (!C::kF32) {
+                        float few_x[16];
+                        if (split) {
+                            tmem_ld16_nowait(sc + 16 * quarter, few_x);
+                            tmem_wait_ld();
+                            past_end(few_x, 16 * quarter, 16);
+#pragma unroll
+                            for (int g = 0; g < 2; ++g) {
+                                const float f = C::kF32 ? factor(2 * quarter + g) : cq;
+                                const float e = C::kF32 ? exponent(2 * quarter + g) : 0.0f;
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    top4[j & 3] = fmaxf(top4[j & 3], C::kF32 ? fmaf(few_x[8 * g + j], f, e)
+                                                                             : few_x[8 * g + j]);
+                                if (score) {
+                                    float4 *o = reinterpret_cast<float4 *>(score + (s.j0 + i) * kTile + 16 * quarter);
+#pragma unroll
+                                    for (int j = 8 * g; j < 8 * g + 8; j += 4)
+                                        o[j >> 2] = make_float4(few_x[j] * f, few_x[j + 1] * f, few_x[j + 2] * f,
+                                                                few_x[j + 3] * f);
+                                }
+                            }
+                        } else if constexpr (!C::kF32) {
                             tmem_ld32_nowait(sc, x);
                             tmem_ld32_nowait(sc + 32, x + 32);
                             tmem_wait_ld();
@@ -1089,12 +1174,14 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
                         if constexpr (!C::kF32) top *= cq;
                         // ---- the reference exponent ----------------------------------------------------
-                        const float want = top == -INFINITY ? (any ? mref : 0.0f) : rintf(top) - kShift;
-                        if (!any) {
-                            mref = want;
-                        } else if (__any_sync(0xffffffffu, want > mref + kGrow)) {
+                        // (a row with no score yet, all of them past the end, takes any: its l and O are 0)
+                        const float want = top == -INFINITY ? mref : rintf(top) - kShift;
+                        const bool grown = any && want > mref + kGrow;
+                        if (!any) mref = want;
+                        any = any || top > -INFINITY;
+                        if (__any_sync(0xffffffffu, grown)) {
                             wait_pv();
-                            const float to = want > mref + kGrow ? want : mref;
+                            const float to = grown ? want : mref;
                             const float f = ex2(mref - to);
                             mref = to;
                             l *= f;
@@ -1122,7 +1209,22 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                                 hi[j >> 1] = split2<typename std::conditional<C::kF32, __half, T>::type>(p, lo[j >> 1]);
                             }
                         };
-                        if constexpr (C::kF32) {
+                        if (split) {
+                            uint32_t w[16], zero[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) zero[j] = 0u;
+#pragma unroll
+                            for (int kk = 1; kk < 4; ++kk) tmem_st16(sc + 16 * ((quarter + kk) & 3), zero);
+#pragma unroll
+                            for (int g = 0; g < 2; ++g) {
+                                const float ev = C::kF32 ? exponent(2 * quarter + g) : 0.0f;
+                                sum2 = make_float2(0.0f, 0.0f);
+                                weigh8(few_x + 8 * g, C::kF32 ? factor(2 * quarter + g) : cq, ev - mref, w + 4 * g,
+                                       w + 8 + 4 * g);
+                                l = fmaf(sum2.x + sum2.y, C::kF32 ? pow2(-(int)ev) : 1.0f, l);
+                            }
+                            tmem_st16(sc + 16 * quarter, w);
+                        } else if constexpr (C::kF32) {
                             auto weigh = [&](float *y, int kk) {
                                 uint32_t w[16];
                                 past_end(y, 16 * kk, 16);
@@ -1157,7 +1259,6 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                             l += sum2.x + sum2.y;
                         }
                         tmem_wait_st();
-                        any = true;
                     }
                     wait_pv();
                     tc_before();
@@ -1230,7 +1331,8 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             top = fmaxf(M, top);
-            const float f = k < np + no ? ex2(x.x - top) : 0.0f, old = k0 ? ex2(M - top) : 0.0f;
+            // (-inf: no score)
+            const float f = x.x > -INFINITY ? ex2(x.x - top) : 0.0f, old = M > -INFINITY ? ex2(M - top) : 0.0f;
             M = top;
             L = fmaf(L, old, warp_sum(x.y * f));
             if (!out) continue;
