@@ -48,6 +48,11 @@
 // p' 2^-e.  m is an integer: x + (e - m) then rounds once, at the size of the
 // exponent that matters.
 //
+// The tensor cores cut every addition to O off towards zero, 12 additions a tile:
+// O came out 1e-5 too small after 64 tiles of a stream.  F32 therefore adds O to
+// a sum in global memory, rounded to nearest, every kFlush tiles and starts it
+// again from zero (and the small products of a tile go first).
+//
 // TMEM columns: S/P buffers 0..63 and 64..127, Q 128.., O up to 511.
 // Every wait is bounded.
 #include <cuda.h>
@@ -69,6 +74,7 @@ constexpr int kFew = 16;             // units of at most so many rows: a tile's 
 constexpr int kPad = 3;              // list places a unit takes beside its tiles: what its segment's ends cost
 constexpr int kLens = 512;           // sequences whose lengths a CTA keeps in shared memory
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (loaders run at most 5 ahead)
+constexpr int kFlush = 4;            // F32: a stream's tiles between two additions of its O to the sum in memory
 constexpr float kShift = 6.0f;       // weights up to 2^6 at the reference maximum, 2^14 before a rescale
 constexpr float kGrow = 8.0f;        // growth of a row's maximum that is left in place
 constexpr int kStageBudget2 = 160 * 1024, kStageBudget1 = 192 * 1024, kStageBudgetRaw = 128 * 1024;
@@ -141,6 +147,7 @@ struct AbArgs {
     int *cum;                    // [n_seq + 1] list places of the sequences before b (one unit each)
     float *part_p, *part_o;      // partial O of prefix and own units
     float2 *ml_p, *ml_o;         // their (m, l)
+    float *sum;                  // F32: [CTA][stream][value column][row] O of the segment's earlier tiles
     float *score;                // add_weights: x_j [n_seq][n_head][pitch]
     float *row_weight;
     void *out;
@@ -354,6 +361,29 @@ __device__ __forceinline__ uint32_t split2(float2 x, uint32_t &lo) {
     return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);   // bf16: the upper halves
 }
 
+// F32's weights and values: the high part is x rounded to fp16, so that the
+// rests have either sign and the product of two rests, which is left out, is 0
+// on average and not 2^-22 of the whole.
+__device__ __forceinline__ uint32_t split_rn(float2 x, uint32_t &lo) {
+    const uint32_t hi = pack2<__half>(x.x, x.y);
+    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    const float2 r = __fadd2_rn(x, make_float2(-h.x, -h.y));
+    lo = pack2<__half>(r.x, r.y);
+    return hi;
+}
+
+// Keys and queries, in (-2^15, 2^15): the high part is x rounded to a multiple
+// of 16 (11 bits), the rest is within 8 and so held to 2^-9.  High parts on one
+// grid make the sums of their products integers below 2^24 in all but the
+// largest scores, which the tensor cores add without cutting anything off.
+__device__ __forceinline__ uint32_t split_grid(float2 x, uint32_t &lo) {
+    const float2 m = make_float2(201326592.0f, 201326592.0f);    // 1.5 x 2^27: its unit is 16
+    const float2 t = __fadd2_rn(x, m), h = __fadd2_rn(t, make_float2(-m.x, -m.y));
+    const float2 r = __fadd2_rn(x, make_float2(-h.x, -h.y));
+    lo = pack2<__half>(r.x, r.y);
+    return pack2<__half>(h.x, h.y);
+}
+
 // Exponent e, 2^e the power of two that v 2^-e puts |v| <= amax below 2^15
 // (and amax at or above 2^14), held in a range where 2^e and 2^-e stay normal.
 __device__ __forceinline__ int part_exponent(float amax) {
@@ -425,7 +455,7 @@ struct RowLoad {
         const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         return part_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
     }
-    __device__ __forceinline__ void store(uint8_t *stage, int r0, float scale, int lane) const {
+    __device__ __forceinline__ void store(uint8_t *stage, int r0, float scale, bool grid, int lane) const {
         constexpr int W = COLS < 64 ? COLS : 64;
         constexpr uint32_t kLo = kTile * COLS * 2;
         const int rr = lane / kLanes, cc = (lane % kLanes) * 4;
@@ -433,8 +463,14 @@ struct RowLoad {
         for (int i = 0; i < kN; ++i) {
             const int r = r0 + i / kVec * kPer + rr, c = cc + (i % kVec) * 4 * kLanes;
             uint2 hi, lo;
-            hi.x = split2<__half>(make_float2(x[i].x * scale, x[i].y * scale), lo.x);
-            hi.y = split2<__half>(make_float2(x[i].z * scale, x[i].w * scale), lo.y);
+            const float2 a = make_float2(x[i].x * scale, x[i].y * scale), b = make_float2(x[i].z * scale, x[i].w * scale);
+            if (grid) {
+                hi.x = split_grid(a, lo.x);
+                hi.y = split_grid(b, lo.y);
+            } else {
+                hi.x = split_rn(a, lo.x);
+                hi.y = split_rn(b, lo.y);
+            }
             const int unit = (c % W) >> 3;
             const int sw = W == 64 ? unit ^ (r & 7) : unit ^ ((r >> 1) & 3);
             const uint32_t off = (uint32_t)(c / W) * (kTile * W * 2) + r * (W * 2) + sw * 16 + (c & 4) * 2;
@@ -606,7 +642,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 const uint32_t st = k / C::kGroups, g = k % C::kGroups, slot = st % C::kStages, use = st / C::kStages;
                 const int e = x.exponent();
                 if (use > 0) ok = ok && warp_wait(&empty[slot], (use - 1) & 1u, a.status);
-                x.store(smem + slot * C::kStage, C::kRows * g, pow2(-e), lane);
+                x.store(smem + slot * C::kStage, C::kRows * g, pow2(-e), !(st & 1), lane);     // even stages: keys
                 // K: the factor that undoes the scaling; V: the exponent
                 if (lane == 0) side[((st >> 1) % kSide) * 16 + (st & 1) * 8 + g] = st & 1 ? (float)e : pow2(e);
                 fence_async();
@@ -752,7 +788,9 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     if constexpr (C::kF32) {
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
-                            mma_f16_ta(d, C::kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS, kk ? 1u : 0u);
+                            mma_f16_ta(d, C::kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS,
+                                       kk ? 1u : 0u);
+                            mma_f16_ta(d, C::kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS, 1u);
                             mma_f16_ta(d, C::kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, 1u);
                         }
                     }
@@ -766,7 +804,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     const int j = i - C::kAhead;
                     // the last segment's O is read by now, or will be soon
                     if (j == 0 && segs > 1 && !(ok = warp_wait(oready, segs & 1u, a.status))) break;
-                    ok = issue_pv(tile + j, j < C::kNS);
+                    const int mine = j / C::kNS;       // the stream's tile of the segment
+                    ok = issue_pv(tile + j, C::kF32 ? mine % kFlush == 0 : mine == 0);
                 }
             }
             tile += n;
@@ -847,9 +886,9 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 for (int u = 0; u < kLpr; ++u) {
                     const uint4 x = *reinterpret_cast<const uint4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4));
                     if constexpr (C::kF32) {
-                        hi[2 * u] = split2<__half>(
+                        hi[2 * u] = split_grid(
                             make_float2(__uint_as_float(x.x) * qs, __uint_as_float(x.y) * qs), lo[2 * u]);
-                        hi[2 * u + 1] = split2<__half>(
+                        hi[2 * u + 1] = split_grid(
                             make_float2(__uint_as_float(x.z) * qs, __uint_as_float(x.w) * qs), lo[2 * u + 1]);
                     } else {
                         // a negative scale turns the queries' signs
@@ -910,13 +949,39 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             return cq;
         };
 
+        // F32: a stream's O, which starts again from zero, added to its sum (the
+        // first time: put there)
+        float *sum = nullptr;
+        float mref = 0.0f, msum = 0.0f;          // reference exponents of O and of the sum
+        if constexpr (C::kF32) sum = a.sum + (size_t)blockIdx.x * C::kNS * C::kDV * kM + row;
+        auto flush = [&](uint32_t stream, bool first) {
+            const float f = ex2(msum - mref);
+            float *p = sum + stream * C::kDV * kM;
+            constexpr int kC = C::kDV < 64 ? C::kDV : 64;    // columns whose sums are loaded together
+#pragma unroll 1
+            for (int c0 = 0; c0 < C::kDV; c0 += kC, p += kC * kM) {
+                float v[kC];
+#pragma unroll
+                for (int k = 0; k < kC; ++k) v[k] = first ? 0.0f : p[k * kM];
+#pragma unroll
+                for (int c = 0; c < kC; c += 16) {
+                    float o[16];
+                    tmem_ld16_nowait(lanes + C::kColO + stream * C::kDV + c0 + c, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) p[(c + k) * kM] = first ? o[k] : fmaf(v[c + k], f, o[k]);
+                }
+            }
+            msum = mref;
+        };
+
         Seg nx;
         int n = 0;                               // the segment's tiles
         bool have = false, had = false;          // a segment is open; one of its tiles was this warpgroup's
         bool active = false;                     // a row of this warp belongs to its unit
         bool split = false;                      // at most 16 rows: this warp has 16 columns of a tile
         bool any = false;                        // this thread's row has met a score
-        float cq = 0.0f, mref = 0.0f, l = 0.0f;
+        float cq = 0.0f, l = 0.0f;
 #pragma unroll 1
         for (;;) {
             // ---- from one segment to the next ------------------------------------------------------
@@ -926,9 +991,15 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             // scores can start while O is read.
             const bool nhave = walk.template next<C::kNDV>(a, list, nx);
             if (nhave) q_begin(nx);
+            // tiles of each stream in the segment
+            const int cnt0 = C::kNS == 1 ? n : (n + 1 - (int)(tile & 1u)) / 2, cnt1 = n - cnt0;
             if (had) {
                 const uint32_t k = C::kNS == 2 ? wg : 0;
                 ok = ok && warp_wait(&ofull[k], ((k ? pv1 : pv0) - 1) & 1u, a.status);
+                if constexpr (C::kF32) {
+                    tc_after();
+                    if (active && (k ? cnt1 : cnt0) > kFlush) flush(k, false);
+                }
             }
             ml[turn * 2 * kM + wg * kM + row] = make_float2(had && any ? mref : -INFINITY, l);
             if (nhave) q_share(nx);
@@ -972,6 +1043,16 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         tmem_ld16_nowait(lanes + C::kColO + c, o);
                         if constexpr (C::kNS == 2) tmem_ld16_nowait(lanes + C::kColO + C::kDV + c, v);
                         tmem_wait_ld();
+                        if constexpr (C::kF32) {       // a stream with more tiles: its sum
+                            if (cnt0 > kFlush) {
+#pragma unroll
+                                for (int k = 0; k < kP; ++k) o[k] = __ldcg(sum + (c + k) * kM);
+                            }
+                            if (C::kNS == 2 && cnt1 > kFlush) {
+#pragma unroll
+                                for (int k = 0; k < kP; ++k) v[k] = __ldcg(sum + (C::kDV + c + k) * kM);
+                            }
+                        }
 #pragma unroll
                         for (int k = 0; k < kP; ++k) {
                             o[k] = has0 ? o[k] * f0 : 0.0f;
@@ -1070,6 +1151,13 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     const int valid = s.n - (s.j0 + i) * kTile;     // of the tile's 64 rows
                     ok = ok && warp_wait(&sfull[buf], (t / C::kBufs) & 1u, a.status);
                     tc_after();
+                    if constexpr (C::kF32) {
+                        const int k = i / C::kNS;       // the stream's tile of the segment
+                        if (k > 0 && k % kFlush == 0) {
+                            wait_pv();
+                            if (active) flush(stream, k == kFlush);
+                        }
+                    }
                     if constexpr (!C::kF32) {
                         // stale rows behind a sequence's end may hold anything, NaN too,
                         // and 0 x NaN is NaN: the values' tile gets zeros there
@@ -1206,7 +1294,10 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                                     __ffma2_rn(make_float2(y[j], y[j + 1]), make_float2(f, f), make_float2(e, e));
                                 const float2 p = make_float2(ex2(v.x), ex2(v.y));
                                 sum2 = __fadd2_rn(sum2, p);
-                                hi[j >> 1] = split2<typename std::conditional<C::kF32, __half, T>::type>(p, lo[j >> 1]);
+                                if constexpr (C::kF32)
+                                    hi[j >> 1] = split_rn(p, lo[j >> 1]);
+                                else
+                                    hi[j >> 1] = split2<T>(p, lo[j >> 1]);
                             }
                         };
                         if (split) {
@@ -1404,7 +1495,7 @@ int ab_shape(const lalb_kv_batch *c, const lalb_attn_batch *p) {
 
 struct Plan {
     AbArgs a;
-    size_t o_cum, o_mlp, o_mlo, o_pp, o_po, o_score, bytes;
+    size_t o_cum, o_mlp, o_mlo, o_pp, o_po, o_sum, o_score, bytes;
 };
 
 void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
@@ -1439,6 +1530,8 @@ void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
     pl->o_mlo = take(so * a.rows_o * sizeof(float2));
     pl->o_pp = take(sp * a.rows_p * dv * sizeof(float));
     pl->o_po = take(so * a.rows_o * dv * sizeof(float));
+    // F32: two streams of 128 value columns at most
+    pl->o_sum = take(c->dtype == LALB_DT_F32 ? (size_t)kGrid * std::min(2 * a.hd, 256) * kM * sizeof(float) : 0);
     pl->o_score = take(a.add_weights ? (size_t)a.n_seq * a.n_head * a.pitch * sizeof(float) : 0);
     pl->bytes = off;
 }
@@ -1513,6 +1606,7 @@ extern "C" int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache, c
     a.ml_o = reinterpret_cast<float2 *>(w + pl.o_mlo);
     a.part_p = reinterpret_cast<float *>(w + pl.o_pp);
     a.part_o = reinterpret_cast<float *>(w + pl.o_po);
+    a.sum = reinterpret_cast<float *>(w + pl.o_sum);
     a.score = reinterpret_cast<float *>(w + pl.o_score);
     a.row_weight = cache->row_weight;
     a.out = out;
