@@ -231,8 +231,8 @@ LALB_API int lalb_rope_append(lalb_ctx *ctx, const lalb_rope *rope, const lalb_k
  * read); the prefix rows' weights are not kept.  q, the caches and out have
  * the cache's type; q row b starts at q + b*q_stride elements.  F32: keys,
  * queries, values and weights enter the tensor cores as two fp16 parts (22
- * bits) under per-row powers of two, products are summed in fp32.  F16 and
- * BF16: weights are rounded to that type before the product with v.  A
+ * bits) under powers of two shared by 16 rows, products are summed in fp32.
+ * F16 and BF16: weights enter as two parts of that type.  A
  * length outside its range counts as 0 and raises status bit 2.  ws: from
  * lalb_attention_batch_ws_bytes, 256-byte aligned, nothing kept between
  * calls; calls that may overlap need one each.  The result does not depend

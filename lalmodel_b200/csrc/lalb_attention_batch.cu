@@ -23,42 +23,58 @@
 // tile, with zeros as the weights of the rest; the four warps' sums are added
 // at the segment's end.
 //
-// Split.  All tiles of all units form one list, and CTA c of G (one per SM)
-// takes tiles [c W / G, (c + 1) W / G): equal shares whatever the lengths,
-// without the host knowing them.  A run of tiles of one unit in one CTA (a
-// segment) ends in one partial; attention_combine_kernel adds a row's partials
-// in list order, so results do not depend on scheduling.
+// Split.  All tiles of all units form one list (List), and every CTA, one per
+// SM, takes an equal run of it: equal shares whatever the lengths, without the
+// host knowing them.  A run of tiles of one unit in one CTA (a segment) ends in
+// one partial; attention_combine_kernel adds a row's partials in list order, so
+// results do not depend on scheduling.
 //
 // One CTA, warp-specialised (kSoftWarps softmax, 1 MMA, the loaders):
 //   loaders  K and V tiles into a ring, in the order K0 V0 K1 V1 ..; 16-bit
 //            caches by tiled TMA straight into the swizzled operand layout;
-//            F32 by eight warps that split each value into two fp16 parts;
-//   MMA      S(j+1) is issued before PV(j), so that the tensor cores work on
+//            F32 rows by TMA to the seven loader warps, which split each value
+//            into two fp16 parts;
+//   MMA      S runs kAhead tiles ahead of PV, so that the tensor cores work on
 //            the next scores while the softmax of this tile runs; Q is the A
 //            operand from TMEM, P overwrites its S in TMEM as the next A;
 //   softmax  two warpgroups on alternate tiles, each with its own O (128 rows
 //            = TMEM lanes = threads, so rows need no shuffles); O is rescaled
-//            only when a row's maximum has grown by more than 2^8.
+//            only when a row's maximum has grown by more than 2^8.  The weights
+//            enter PV as two parts, so that they are not rounded to the
+//            cache's type (one part: 1.4 times the output error).
 //
-// F32: x = hi + lo in fp16 (22 bits), three of the four products.  The rows of
-// a tile that a loader warp splits at a time share a power of two that puts
-// their largest |x| in [2^14, 2^15); K's goes into the scores' factor, V's
-// exponent e into the weights' exponent: p' = 2^(x + e - m), v' = v 2^-e, so
-// that p' keeps its precision whatever the values' range, and l takes
-// p' 2^-e.  m is an integer: x + (e - m) then rounds once, at the size of the
-// exponent that matters.
+// F32: x = hi + lo in fp16 (22 bits).  The rows of a tile that a loader warp
+// splits at a time share a power of two that puts their largest |x| in
+// [2^14, 2^15); K's goes into the scores' factor, V's exponent e into the
+// weights' exponent: p' = 2^(x + e - m), v' = v 2^-e, so that p' keeps its
+// precision whatever the values' range, and l takes p' 2^-e.  m is an integer:
+// x + (e - m) then rounds once, at the size of the exponent that matters.
 //
-// The tensor cores cut every addition to O off towards zero, 12 additions a tile:
-// O came out 1e-5 too small after 64 tiles of a stream.  F32 therefore adds O to
-// a sum in global memory, rounded to nearest, every kFlush tiles and starts it
-// again from zero (and the small products of a tile go first).
+// The tensor cores cut every addition to an accumulator off towards zero.  In S
+// the three small products go first, while the sum is small, and the large ones
+// add up exactly (split_grid).  O, 12 additions a tile, came out 1e-5 too
+// small after 64 tiles of a stream: F32 adds it to a sum in global memory,
+// rounded to nearest, every kFlush tiles and starts it again from zero.
 //
-// TMEM columns: S/P buffers 0..63 and 64..127, Q 128.., O up to 511.
-// Every wait is bounded.
+// What bounds it (B200; bytes and products that it cannot do without against the
+// measured 6540 GB/s and 1637 TFLOP/s; a pass from a graph, caches warm):
+//   64 sequences, 16384 + 0..1000 bf16 rows, 28 heads on 4 of 128: 52 us; the
+//     memory floor is 15 us, the tensor floor (three products' time for two)
+//     14; tiles come from L2 at 6.4 TB/s, 32 KB for 128 query rows, as fast
+//     as the softmax warps weigh them (0.9 us a tile), and the ends of some 400
+//     segments cost 3 us each;
+//   16 sequences, 4093 + 1..700 F32 rows: 33 us, floor 6; one tile takes its
+//     CTA 2 us, most of it in the loaders' splitting and the softmax's waits;
+//   8 sequences, 3001..8191 f16 rows, 16 heads on 8 of 64: 40 us, floor 14;
+//   one sequence of 812 F32 rows: 16 us, of which each CTA's single tile takes 8
+//     from launch to partial, all latency: lengths, Q, rows, S, weights, PV in turn.
+//
+// TMEM columns: S/P buffers from 0, then Q, O up to 511.  Every wait is bounded.
 #include <cuda.h>
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "lalb_batch.cuh"
 #include "lalb_tcgen05.cuh"
@@ -73,8 +89,11 @@ constexpr int kM = 128;              // query rows per unit
 constexpr int kFew = 16;             // units of at most so many rows: a tile's columns are split over the warps
 constexpr int kPad = 3;              // list places a unit takes beside its tiles: what its segment's ends cost
 constexpr int kLens = 512;           // sequences whose lengths a CTA keeps in shared memory
-constexpr int kSide = 8;             // tiles whose F32 scales are kept (loaders run at most 5 ahead)
-constexpr int kFlush = 4;            // F32: a stream's tiles between two additions of its O to the sum in memory
+constexpr int kSide = 8;             // tiles whose F32 scales are kept (Cfg checks that they outlive the ring)
+// F32: a stream's tiles between two additions of its O to the sum in memory (1, 2,
+// 4: 41, 37, 31 us for 16 sequences behind 4093 rows; output errors of 1024 rows
+// 0.9, 1.1 and 1.5e-6 before keys and queries were split on a grid)
+constexpr int kFlush = 4;
 constexpr float kShift = 6.0f;       // weights up to 2^6 at the reference maximum, 2^14 before a rescale
 constexpr float kGrow = 8.0f;        // growth of a row's maximum that is left in place
 constexpr int kStageBudget2 = 160 * 1024, kStageBudget1 = 192 * 1024, kStageBudgetRaw = 128 * 1024;
@@ -153,7 +172,7 @@ struct AbArgs {
     void *out;
     unsigned int *status;
     long long q_stride;
-    int n_seq, n_head, n_kv, group, hd, max_ctx, prefix, add_weights;
+    int n_seq, n_head, n_kv, group, max_ctx, prefix, add_weights;
     int m_p, m_o;                // 128-row tiles of a prefix and an own unit's KV head
     int rows_p, rows_o;          // rows kept per partial: query rows of a prefix and an own unit at most
     int pitch;
@@ -172,7 +191,9 @@ __device__ __forceinline__ int checked_len(const AbArgs &a, int n) { return n < 
 // CTA c takes `per` places, the first `rem` CTAs one more.  A segment's ends
 // (Q, the pipeline's fill and drain, the partial) take as long as about three
 // tiles; without empty places for them, CTAs with many short units finish last
-// (64 sequences of 500 rows behind a prefix of 16384: 69 us, with them see below).
+// (64 sequences of up to 1000 rows behind a prefix of 16384, bf16: 69 us, with
+// 3 places 52, with 2 or 4 60 and 54; 30 F32 sequences of up to 1000: 39, 39
+// and 46 with 3, 2 and 4).
 // (The host bounds every index.)
 struct List {
     int tp, total;         // places of the prefix units, all places
@@ -1505,7 +1526,6 @@ void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
     a.n_head = p->n_head;
     a.n_kv = c->n_kv_head;
     a.group = p->n_head / c->n_kv_head;
-    a.hd = c->head_dim;
     a.max_ctx = c->max_ctx;
     a.prefix = p->prefix_len;
     a.add_weights = p->add_weights != 0;
@@ -1515,7 +1535,7 @@ void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
     a.rows_p = std::min(kM, a.n_seq * a.group);
     a.rows_o = std::min(kM, a.group);
     a.pitch = tiles_of(a.max_ctx) * kTile;
-    const int dv = a.hd / ndv;
+    const int hd = c->head_dim, dv = hd / ndv;
     // a segment's slot is its CTA's number plus its unit's
     const size_t sp = a.prefix ? (size_t)kGrid + (size_t)a.n_kv * a.m_p * ndv : 0;
     const size_t so = (size_t)kGrid + (size_t)a.n_seq * a.n_kv * a.m_o * ndv;
@@ -1531,7 +1551,7 @@ void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
     pl->o_pp = take(sp * a.rows_p * dv * sizeof(float));
     pl->o_po = take(so * a.rows_o * dv * sizeof(float));
     // F32: two streams of 128 value columns at most
-    pl->o_sum = take(c->dtype == LALB_DT_F32 ? (size_t)kGrid * std::min(2 * a.hd, 256) * kM * sizeof(float) : 0);
+    pl->o_sum = take(c->dtype == LALB_DT_F32 ? (size_t)kGrid * std::min(2 * hd, 256) * kM * sizeof(float) : 0);
     pl->o_score = take(a.add_weights ? (size_t)a.n_seq * a.n_head * a.pitch * sizeof(float) : 0);
     pl->bytes = off;
 }
@@ -1539,13 +1559,16 @@ void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
 struct Kernels {
     const void *tiles, *combine;
     int threads, smem, rows;
+    int regs;                      // a thread at launch, which the roles' split shares out
+    std::atomic<int> *checked;     // the kernel's register count as loaded, once read
 };
 
 template <class T, int HD>
 Kernels kernels_of() {
     using C = Cfg<T, HD>;
+    static std::atomic<int> checked{0};
     return {(const void *)attention_tiles_kernel<T, HD>, (const void *)attention_combine_kernel<T, HD>, C::kThreads,
-            (int)C::kSmem, C::kRows};
+            (int)C::kSmem, C::kRows, C::kSoftRegs ? C::kEven : 0, &checked};
 }
 
 template <class T>
@@ -1619,17 +1642,31 @@ extern "C" int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache, c
     a.decay = attn->decay;
     DeviceGuard guard(ctx->device);
     if (!guard.ok()) return lalb_fail(ctx, LALB_ERR_CUDA, "attention_batch: device %d", ctx->device);
-    const Kernels kn = cache->dtype == LALB_DT_F32   ? kernels_for<float>(a.hd)
-                       : cache->dtype == LALB_DT_F16 ? kernels_for<__half>(a.hd)
-                                                     : kernels_for<__nv_bfloat16>(a.hd);
+    const int hd = cache->head_dim;
+    const Kernels kn = cache->dtype == LALB_DT_F32   ? kernels_for<float>(hd)
+                       : cache->dtype == LALB_DT_F16 ? kernels_for<__half>(hd)
+                                                     : kernels_for<__nv_bfloat16>(hd);
     if (int st = lalb_set_smem_attr(ctx, kn.tiles, kn.smem)) return st;
+    // a block launched with fewer registers than its roles ask for would wait for them for good
+    if (kn.regs) {
+        int regs = kn.checked->load(std::memory_order_relaxed);
+        if (!regs) {
+            cudaFuncAttributes attr;
+            LALB_CUDA_TRY(ctx, cudaFuncGetAttributes(&attr, kn.tiles));
+            regs = attr.numRegs;
+            kn.checked->store(regs, std::memory_order_relaxed);
+        }
+        if (regs < kn.regs)
+            return lalb_fail(ctx, LALB_ERR_UNSUPPORTED, "attention_batch: kernel built with %d registers of %d", regs,
+                             kn.regs);
+    }
     CUtensorMap maps[4] = {};
     {
         // 16 bits: swizzled 64-column tiles of 64 rows; F32: a loader warp's plain rows of a head
         const CUtensorMapDataType dt = es == 4                         ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                        : cache->dtype == LALB_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        const int box = es == 4 ? a.hd : std::min(64, a.hd), rows_box = es == 4 ? kn.rows : kTile;
+        const int box = es == 4 ? hd : std::min(64, hd), rows_box = es == 4 ? kn.rows : kTile;
         const CUtensorMapSwizzle sw = es == 4     ? CU_TENSOR_MAP_SWIZZLE_NONE
                                       : box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B
                                                   : CU_TENSOR_MAP_SWIZZLE_64B;
@@ -1637,7 +1674,7 @@ extern "C" int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache, c
         for (int i = 0; i < 4; ++i) {
             const long long rows = i < 2 ? a.prefix : (long long)a.n_seq * a.max_ctx;
             if (rows == 0) continue;
-            if (int st = map2d(ctx, &maps[i], base[i], dt, es, (long long)a.n_kv * a.hd, rows, box, rows_box, sw))
+            if (int st = map2d(ctx, &maps[i], base[i], dt, es, (long long)a.n_kv * hd, rows, box, rows_box, sw))
                 return st;
         }
     }

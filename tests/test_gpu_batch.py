@@ -151,23 +151,28 @@ def test_rope_append_bad_slot_is_reported(ctx):
 # ---- attention ------------------------------------------------------------------------------
 def score_step(top):
     """Bound on a score's error in natural units, from sum |q k| * scale:
-    operands are exact (16 bits) or within 2^-22 each (two fp16 parts, with the
-    product of the low parts, 2^-22, left out): 3 x 2^-22; at most 48 fp32
-    additions on the tensor cores (head_dim 256: 16 steps of each of 3
-    products) within 2^-23 each; scale and shift round twice: 64 x 2^-23."""
+    operands are exact (16 bits) or two fp16 parts, the high one on a grid of
+    2^-11 of the largest of 16 rows, the rest within 2^-24 of it: 2 x 2^-23 of
+    sum |q k| for the sizes tested; at most 16 large fp32 additions on the
+    tensor cores (head_dim 256) within 2^-23 each, the 48 of the small products
+    2^-10 of that; scale and shift round twice; twice all that: 64 x 2^-23."""
     return top * 64 * 2.0 ** -23
 
 
 def attn_tol(ref, mag, top, dt, rows):
     """p is off by twice the score's error (its own and the maximum's) and by
-    exp2's 2 ulp; the sums over rows add at most 2^-23 per 16 rows each; the
-    split weights and values are within 3 x 2^-22; 16-bit weights round by
-    half a step, the output by another."""
+    exp2's 2 ulp (2^-22); weights and values as two fp16 parts are within 3 x
+    2^-22.  The tensor cores cut each addition off by up to 2^-23 of the sum:
+    F32 makes 12 a tile of 64 rows, in runs of 4 tiles whose sums are then added
+    in fp32 (one rounding per 256 rows); 16 bits makes 8 a tile.  8 more
+    roundings join streams and partials.  16-bit outputs round by half a step
+    (and their weights, as two parts, by its square)."""
     hd = ref.shape[1] // top.shape[1]
     t = top.repeat_interleave(hd, 1)
-    rel = 2 * score_step(t) + 2.0 ** -21 + (rows / 16 + 8) * 2.0 ** -23
+    adds = min(rows * 12 / 64, 48) + rows / 256 if dt == torch.float32 else rows * 8 / 64
+    rel = 2 * score_step(t) + 2.0 ** -22 + 3 * 2.0 ** -22 + (adds + 8) * 2.0 ** -23
     if dt != torch.float32:
-        rel = rel + half_step(dt)
+        rel = rel + half_step(dt) ** 2 * 4
     tiny = 0 if dt == torch.float32 else 2.0 ** -25
     return mag * rel * (1 + half_step(dt)) + half_step(dt) * ref.abs() + tiny
 
@@ -197,7 +202,9 @@ def run_attention(ctx, dtype, B, nh, nk, hd, L, lens, C, seed, weights=None, sca
         live = torch.arange(C)[None, None, :] < n[:, None, None]
         want = torch.where(live, weights * w0.double() + w, w0.double())
         step = score_step(top).view(B, nk, -1).amax(-1)[:, :, None]
-        tol = torch.where(live, w * (2 * step + 2.0 ** -21 + (rows / 16 + 8) * 2.0 ** -23)
+        # the sum of exponentials is added up in fp32: a rounding per row of a
+        # tile's 64 on each of its paths at most, one per tile and partial
+        tol = torch.where(live, w * (2 * step + 2.0 ** -21 + (64 + rows / 64 + 8) * 2.0 ** -24)
                           + 3 * 2.0 ** -24 * want.abs() + 1e-38, torch.zeros_like(want))
         within(cache.row_weight, want, tol)
     return out, cache
@@ -259,6 +266,47 @@ def test_attention_batch_f32_ranges(ctx, mag):
     out = ctx.attention_batch(cache, (q * mag).cuda(), lens.cuda(), nh, (pk / mag).cuda(), pv.cuda())
     ref, _, m, top = R.attention((q * mag), kc.cpu(), v, lens, nh, nk, (pk / mag), pv)
     within(out, ref, attn_tol(ref, m, top, torch.float32, L + 80))
+
+
+@pytest.mark.parametrize("dtype,hd,nk,nh,B,L,C", [
+    ("f32", 32, 8, 8, 2, 12000, 40),      # several sums of O per segment, few rows
+    ("f32", 128, 1, 8, 20, 40000, 9),     # .. and 160 rows of queries
+    ("f32", 256, 2, 2, 3, 20000, 70),     # one stream of tiles
+    ("bf16", 64, 4, 8, 3, 30000, 70),
+])
+def test_attention_batch_long(ctx, dtype, hd, nk, nh, B, L, C):
+    run_attention(ctx, dtype, B, nh, nk, hd, L, ints(*[(7 * b + 3) % (C + 1) for b in range(B)]), C, seed=hd, weights=1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attention_batch_many_sequences(ctx, dtype):
+    """More sequences than a CTA keeps lengths of, most of them short, some empty."""
+    B, C = 700, 130
+    lens = torch.tensor([(b * 37) % 9 if b % 50 else C - b % 3 for b in range(B)], dtype=torch.int32)
+    run_attention(ctx, dtype, B, 2, 1, 64, 65, lens, C, seed=5, weights=0.5, stale=float("nan"))
+
+
+def test_attention_batch_two_calls_at_once(ctx):
+    """Two streams, a workspace each, the same cache."""
+    B, nh, nk, hd, C, L = 6, 8, 2, 128, 500, 3000
+    k, v = rand(1, B, C, nk * hd), rand(2, B, C, nk * hd)
+    pk, pv, lens = rand(3, L, nk * hd), rand(4, L, nk * hd), ints(500, 3, 0, 77, 128, 499)
+    cache = lb.KVBatch(k.cuda(), v.cuda(), nk)
+    qs = [rand(10 + i, B, nh * hd) for i in range(2)]
+    dev = [q.cuda() for q in qs]
+    pkd, pvd, ld = pk.cuda(), pv.cuda(), lens.cuda()
+    ws = [ctx.attention_batch_ws(cache, nh, L) for _ in range(2)]
+    outs = [torch.empty_like(d) for d in dev]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                ctx.attention_batch(cache, dev[i], ld, nh, pkd, pvd, ws=ws[i], out=outs[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        ref, _, mag, top = R.attention(qs[i], k, v, lens, nh, nk, pk, pv)
+        within(outs[i], ref, attn_tol(ref, mag, top, torch.float32, L + C))
 
 
 def test_attention_batch_large_scores(ctx):
