@@ -146,8 +146,13 @@ bool rope_turns(const lalb_rope *r, int rot, double *turns) {
         !(r->orig_ctx > 0.0f && std::isfinite(r->orig_ctx) && std::isfinite(r->turns_fast) &&
           std::isfinite(r->turns_slow) && r->turns_fast > r->turns_slow))
         return false;
+    // eight pow calls at most take as long as the rest of the call on the host:
+    // between them the frequencies go on by multiplication (15 roundings, 2^-49)
+    const double step = pow(theta, -2.0 / rot);
+    double power = 1.0;
     for (int d = 0; d < rot / 2; ++d) {
-        double f = pow(theta, -2.0 * d / rot);
+        power = d % 16 ? power * step : pow(theta, -2.0 * d / rot);
+        double f = power;
         if (r->scaling == LALB_ROPE_LINEAR) f /= (double)r->factor;
         if (r->scaling == LALB_ROPE_PARTS) {
             const double t = (double)r->orig_ctx * f / two_pi;
