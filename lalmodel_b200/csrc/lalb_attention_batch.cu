@@ -1432,13 +1432,26 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
         float M = -INFINITY, L = 0.0f, acc[kVec];
 #pragma unroll
         for (int k = 0; k < kVec; ++k) acc[k] = 0.0f;
+        float v[kCombUnroll][kVec];
+        auto fetch = [&](int k0, int m) {       // O of partials k0 .. k0 + kCombUnroll - 1, m of them there
+#pragma unroll
+            for (int j = 0; j < kCombUnroll; ++j) {
+                const int kk = k0 + j;
+                const float *p = kk < np ? a.part_p + (r0p + (size_t)kk * a.rows_p) * C::kDV
+                                         : a.part_o + (r0o + (size_t)(kk - np) * a.rows_o) * C::kDV;
+#pragma unroll
+                for (int q = 0; q < kVec; ++q) v[j][q] = j < m ? __ldcg(p + lane + 32 * q) : 0.0f;
+            }
+        };
+#pragma unroll 1
         for (int k0 = 0; k0 < np + no; k0 += 32) {
-            const int k = k0 + lane;
+            const int k = k0 + lane, m = min(32, np + no - k0);
             float2 x = make_float2(-INFINITY, 0.0f);
             if (k < np)
                 x = __ldcg(a.ml_p + r0p + (size_t)k * a.rows_p);
             else if (k < np + no)
                 x = __ldcg(a.ml_o + r0o + (size_t)(k - np) * a.rows_o);
+            if (out) fetch(k0, m);              // on their way together with (m, l)
             float top = x.x;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -1450,18 +1463,9 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
             if (!out) continue;
 #pragma unroll
             for (int q = 0; q < kVec; ++q) acc[q] *= old;
-            const int m = min(32, np + no - k0);
 #pragma unroll 1
             for (int j0 = 0; j0 < m; j0 += kCombUnroll) {
-                float v[kCombUnroll][kVec];
-#pragma unroll
-                for (int j = 0; j < kCombUnroll; ++j) {
-                    const int kk = k0 + j0 + j;
-                    const float *p = kk < np ? a.part_p + (r0p + (size_t)kk * a.rows_p) * C::kDV
-                                             : a.part_o + (r0o + (size_t)(kk - np) * a.rows_o) * C::kDV;
-#pragma unroll
-                    for (int q = 0; q < kVec; ++q) v[j][q] = j0 + j < m ? __ldcg(p + lane + 32 * q) : 0.0f;
-                }
+                if (j0) fetch(k0 + j0, m - j0);
 #pragma unroll
                 for (int j = 0; j < kCombUnroll; ++j) {
                     const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
