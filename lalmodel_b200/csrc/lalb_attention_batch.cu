@@ -131,6 +131,7 @@ struct Cfg {
     static_assert(kSoftRegs == 0 || kSoftRegs * kSoftWarps + kOtherRegs * kOtherWarps <=
                                         kEven * (kSoftWarps + kOtherWarps),
                   "the split is no more than the block was launched with");
+    static constexpr bool kGrid4 = HD == 256;          // F32: keys and queries on a grid, all four products
     static constexpr uint32_t kStage = kTile * HD * (kF32 ? 4 : 2);
     // F32 rows come in raw, a group at a time, into a slot of the loader warp
     // that splits them (head_dim 256 has no room: plain loads)
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 const uint32_t st = k / C::kGroups, g = k % C::kGroups, slot = st % C::kStages, use = st / C::kStages;
                 const int e = x.exponent();
                 if (use > 0) ok = ok && warp_wait(&empty[slot], (use - 1) & 1u, a.status);
-                x.store(smem + slot * C::kStage, C::kRows * g, pow2(-e), !(st & 1), lane);     // even stages: keys
+                x.store(smem + slot * C::kStage, C::kRows * g, pow2(-e), C::kGrid4 && !(st & 1), lane);     // even stages: keys
                 // K: the factor that undoes the scaling; V: the exponent
                 if (lane == 0) side[((st >> 1) % kSide) * 16 + (st & 1) * 8 + g] = st & 1 ? (float)e : pow2(e);
                 fence_async();
@@ -809,9 +810,11 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     if constexpr (C::kF32) {
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
-                            mma_f16_ta(d, C::kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS,
-                                       kk ? 1u : 0u);
-                            mma_f16_ta(d, C::kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS, 1u);
+                            if constexpr (C::kGrid4)
+                                mma_f16_ta(d, C::kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS,
+                                           kk ? 1u : 0u);
+                            mma_f16_ta(d, C::kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS,
+                                       kk || C::kGrid4 ? 1u : 0u);
                             mma_f16_ta(d, C::kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, 1u);
                         }
                     }
@@ -907,10 +910,10 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 for (int u = 0; u < kLpr; ++u) {
                     const uint4 x = *reinterpret_cast<const uint4 *>(scratch + lane * 128 + ((u ^ (lane & 7)) << 4));
                     if constexpr (C::kF32) {
-                        hi[2 * u] = split_grid(
-                            make_float2(__uint_as_float(x.x) * qs, __uint_as_float(x.y) * qs), lo[2 * u]);
-                        hi[2 * u + 1] = split_grid(
-                            make_float2(__uint_as_float(x.z) * qs, __uint_as_float(x.w) * qs), lo[2 * u + 1]);
+                        const float2 a0 = make_float2(__uint_as_float(x.x) * qs, __uint_as_float(x.y) * qs);
+                        const float2 a1 = make_float2(__uint_as_float(x.z) * qs, __uint_as_float(x.w) * qs);
+                        hi[2 * u] = C::kGrid4 ? split_grid(a0, lo[2 * u]) : split_rn(a0, lo[2 * u]);
+                        hi[2 * u + 1] = C::kGrid4 ? split_grid(a1, lo[2 * u + 1]) : split_rn(a1, lo[2 * u + 1]);
                     } else {
                         // a negative scale turns the queries' signs
                         const uint32_t f = qs < 0.0f ? 0x80008000u : 0u;
