@@ -51,8 +51,9 @@
 // x + (e - m) then rounds once, at the size of the exponent that matters.
 //
 // The tensor cores cut every addition to an accumulator off towards zero.  In S
-// the three small products go first, while the sum is small, and the large ones
-// add up exactly (split_grid).  O, 12 additions a tile, came out 1e-5 too
+// the small products go first, while the sum is small (at head_dim 256 with the
+// product of the two rests, and with high parts whose products add up exactly:
+// split_grid).  O, 12 additions a tile, came out 1e-5 too
 // small after 64 tiles of a stream: F32 adds it to a sum in global memory,
 // rounded to nearest, every kFlush tiles and starts it again from zero.
 //
@@ -63,8 +64,11 @@
 //     14; tiles come from L2 at 6.4 TB/s, 32 KB for 128 query rows, as fast
 //     as the softmax warps weigh them (0.9 us a tile), and the ends of some 400
 //     segments cost 3 us each;
-//   16 sequences, 4093 + 1..700 F32 rows: 33 us, floor 6; one tile takes its
+//   16 sequences, 4093 + 1..700 F32 rows: 31 us, floor 6; one tile takes its
 //     CTA 2 us, most of it in the loaders' splitting and the softmax's waits;
+//   5 sequences, 333 + 100..2000 F32 rows at head_dim 256: 47 us, floor 7; the
+//     ring holds three stages of 64 KB, so that a tile's keys are split only
+//     after the values before the last are used: 4.5 us a tile;
 //   8 sequences, 3001..8191 f16 rows, 16 heads on 8 of 64: 40 us, floor 14;
 //   one sequence of 812 F32 rows: 16 us, of which each CTA's single tile takes 8
 //     from launch to partial, all latency: lengths, Q, rows, S, weights, PV in turn.
@@ -91,8 +95,8 @@ constexpr int kPad = 3;              // list places a unit takes beside its tile
 constexpr int kLens = 512;           // sequences whose lengths a CTA keeps in shared memory
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (Cfg checks that they outlive the ring)
 // F32: a stream's tiles between two additions of its O to the sum in memory (1, 2,
-// 4: 41, 37, 31 us for 16 sequences behind 4093 rows; output errors of 1024 rows
-// 0.9, 1.1 and 1.5e-6 before keys and queries were split on a grid)
+// 4: 41, 37, 31 us for 16 sequences behind 4093 rows, and output errors of 0.9,
+// 1.1 and 1.5e-6 over 1024 rows when parts were still cut off; now 1.1 with 4)
 constexpr int kFlush = 4;
 constexpr float kShift = 6.0f;       // weights up to 2^6 at the reference maximum, 2^14 before a rescale
 constexpr float kGrow = 8.0f;        // growth of a row's maximum that is left in place
@@ -131,7 +135,10 @@ struct Cfg {
     static_assert(kSoftRegs == 0 || kSoftRegs * kSoftWarps + kOtherRegs * kOtherWarps <=
                                         kEven * (kSoftWarps + kOtherWarps),
                   "the split is no more than the block was launched with");
-    static constexpr bool kGrid4 = HD == 256;          // F32: keys and queries on a grid, all four products
+    // F32 keys and queries on a grid, all four products: at head_dim 256 the
+    // output error goes from 2.0 to 0.9e-6 of the whole; at 128 it would go from
+    // 1.1 to 0.9 (1024 rows) for 2 of 33 us (16 sequences behind 4093 rows)
+    static constexpr bool kGrid4 = HD == 256;
     static constexpr uint32_t kStage = kTile * HD * (kF32 ? 4 : 2);
     // F32 rows come in raw, a group at a time, into a slot of the loader warp
     // that splits them (head_dim 256 has no room: plain loads)
@@ -660,9 +667,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 k += C::kLoadWarps;
                 return true;
             };
-            auto finish = [&](const auto &x, int k) {
+            auto finish = [&](const auto &x, int k, int e) {
                 const uint32_t st = k / C::kGroups, g = k % C::kGroups, slot = st % C::kStages, use = st / C::kStages;
-                const int e = x.exponent();
                 if (use > 0) ok = ok && warp_wait(&empty[slot], (use - 1) & 1u, a.status);
                 x.store(smem + slot * C::kStage, C::kRows * g, pow2(-e), C::kGrid4 && !(st & 1), lane);     // even stages: keys
                 // K: the factor that undoes the scaling; V: the exponent
@@ -697,8 +703,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     ok = warp_wait(&bar[slot], (taken / C::kSlots) & 1u, a.status);
                     RowLoad<HD, C::kRows> x;
                     x.load_raw(raw + slot * C::kGroup, left, lane);
+                    const int e = x.exponent();      // the warp's maximum: every lane has its rows
                     ++taken;
-                    __syncwarp();
                     if (issued == taken + C::kSlots - 1 && advance(t)) {
                         issue(t, slot);
                         ++issued;
@@ -707,7 +713,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         else
                             q0 = t;
                     }
-                    finish(x, kk);
+                    finish(x, kk, e);
                 }
                 // nothing may still be on its way into this CTA's shared memory when it ends
                 for (; taken < issued; ++taken) (void)warp_wait(&bar[taken % C::kSlots], (taken / C::kSlots) & 1u, a.status);
@@ -717,11 +723,11 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     if (t.k / C::kGroups & 1) {
                         RowLoad<C::kDV, C::kRows> x;
                         x.load(t.p, pitch, t.left, lane);
-                        finish(x, t.k);
+                        finish(x, t.k, x.exponent());
                     } else {
                         RowLoad<HD, C::kRows> x;
                         x.load(t.p, pitch, t.left, lane);
-                        finish(x, t.k);
+                        finish(x, t.k, x.exponent());
                     }
                 }
             }
