@@ -171,7 +171,7 @@ LALB_API int lalb_attention_decode(lalb_ctx *ctx, const float *qkv, int n_head, 
  * [max_ctx]): eviction keeps different rows for each KV head, so a row's
  * position is known per head.  Rows may be in any order (their keys are
  * already rotated).  All buffers are device memory of the caller; k and v
- * 16-byte aligned.  head_dim 32, 64, 128 or 256; n_seq*max_ctx < 2^31. */
+ * 16-byte aligned.  head_dim 32, 64, 128 or 256; n_seq*max_ctx <= 2^31 - 256. */
 typedef struct {
     int dtype;               /* LALB_DT_F32, LALB_DT_F16 or LALB_DT_BF16 */
     int n_seq, max_ctx, n_kv_head, head_dim;

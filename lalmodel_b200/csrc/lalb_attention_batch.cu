@@ -1515,6 +1515,8 @@ int ab_shape(const lalb_kv_batch *c, const lalb_attn_batch *p) {
     if (int st = kv_batch_shape(c)) return st;
     if (!p || p->prefix_len < 0) return LALB_ERR_INVALID;
     if (int st = lalb_attention_check(p->n_head, c->n_kv_head, c->head_dim)) return st;
+    // a row number rounded up to a tile stays in 31 bits
+    if (p->prefix_len > (1 << 30) || c->max_ctx > (1 << 30)) return LALB_ERR_UNSUPPORTED;
     const long long group = p->n_head / c->n_kv_head;
     if (group > kMaxGroup || (long long)p->n_head * c->head_dim > (1 << 24) || c->n_seq > 65535 ||
         c->n_kv_head > 65535)
@@ -1651,6 +1653,7 @@ extern "C" int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache, c
     const double scale = attn->scale == 0.0f ? 1.0 / sqrt((double)cache->head_dim) : (double)attn->scale;
     // kept away from 0, where (masked) -inf x 0 would be NaN
     a.c = (float)std::max(1e-37, fabs(scale) * 1.4426950408889634074);
+    if (!std::isfinite(a.c)) return lalb_fail(ctx, LALB_ERR_INVALID, "attention_batch: scale %g", scale);
     a.sign = scale < 0.0 ? -1.0f : 1.0f;
     a.decay = attn->decay;
     DeviceGuard guard(ctx->device);

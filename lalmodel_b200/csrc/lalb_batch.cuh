@@ -38,7 +38,8 @@ inline int dtype_size(int dtype) {
 // Shape and type of a cache (no pointers): LALB_OK or the reason's status.
 inline int kv_batch_shape(const lalb_kv_batch *c) {
     if (!c || c->n_seq <= 0 || c->max_ctx <= 0 || c->n_kv_head <= 0) return LALB_ERR_INVALID;
-    if ((long long)c->n_seq * c->max_ctx > 0x7fffffffll) return LALB_ERR_UNSUPPORTED;
+    // row numbers, and those of a tile that begins at the last row, fit 31 bits
+    if ((long long)c->n_seq * c->max_ctx > 0x7fffff00ll) return LALB_ERR_UNSUPPORTED;
     if (!dtype_size(c->dtype)) return LALB_ERR_UNSUPPORTED;
     if (int st = lalb_attention_check(c->n_kv_head, c->n_kv_head, c->head_dim)) return st;
     // a row's elements, and so every index within one, fit 31 bits
@@ -49,7 +50,7 @@ inline int kv_batch_shape(const lalb_kv_batch *c) {
 inline int kv_batch_check(lalb_ctx *ctx, const lalb_kv_batch *c, const char *who) {
     if (int st = kv_batch_shape(c))
         return lalb_fail(ctx, st, "%s: cache (dtype F32, F16 or BF16; head_dim 32, 64, 128 or 256; positive "
-                                  "sizes, n_seq*max_ctx < 2^31)", who);
+                                  "sizes, n_seq*max_ctx <= 2^31 - 256)", who);
     if (!c->k || !c->v || (((uintptr_t)c->k | (uintptr_t)c->v) & 15u))
         return lalb_fail(ctx, LALB_ERR_INVALID, "%s: k and v must be 16-byte aligned device buffers", who);
     if ((((uintptr_t)c->row_pos | (uintptr_t)c->row_weight) & 3u))

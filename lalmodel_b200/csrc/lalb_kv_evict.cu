@@ -384,7 +384,6 @@ extern "C" int lalb_kv_evict(lalb_ctx *ctx, const lalb_kv_batch *cache, int32_t 
         return lalb_fail(ctx, LALB_ERR_INVALID, "kv_evict: misaligned buffer");
     const long long bg = (long long)cache->n_seq * cache->n_kv_head;
     if (bg > 65535) return lalb_fail(ctx, LALB_ERR_UNSUPPORTED, "kv_evict: %lld sequences x KV heads", bg);
-    if (keep == cache->max_ctx) return LALB_OK;   // nothing can be longer
     EvictArgs a = {};
     a.lens = lens;
     a.row_pos = cache->row_pos;

@@ -29,6 +29,11 @@ def test_batch_ws_bytes_host_only():
         assert L.lalb_kv_evict_ws_bytes(cache(**bad), 1, ctypes.byref(n)) == -1
     for bad in (dict(n_head=3), dict(n_head=0), dict(prefix=-1)):
         assert L.lalb_attention_batch_ws_bytes(cache(), attn(**bad), ctypes.byref(n)) == -1
+    # more rows, query rows or tiles than 31-bit indices hold
+    for bad in (dict(n_seq=1, max_ctx=2 ** 31 - 1), dict(n_seq=1, max_ctx=2 ** 30 + 1)):
+        assert L.lalb_attention_batch_ws_bytes(cache(**bad), attn(), ctypes.byref(n)) == -4
+    assert L.lalb_attention_batch_ws_bytes(cache(), attn(prefix=2 ** 31 - 1), ctypes.byref(n)) == -4
+    assert L.lalb_attention_batch_ws_bytes(cache(n_seq=70000, max_ctx=8), attn(), ctypes.byref(n)) == -4
     for keep in (0, 65):
         assert L.lalb_kv_evict_ws_bytes(cache(), keep, ctypes.byref(n)) == -1
     assert L.lalb_kv_evict_ws_bytes(cache(), 8, None) == -1

@@ -420,6 +420,11 @@ def test_kv_evict_bad_length_is_reported_and_left(ctx):
     assert ctx.device_status(reset=True) == BAD_ROW
     assert ld.cpu().tolist() == [21, 10, -3]
     assert torch.equal(cache.k.cpu()[[0, 2]], k[[0, 2]]) and torch.equal(cache.row_weight.cpu()[[0, 2]], w[[0, 2]])
+    # nothing can be too long for a budget of the whole cache, but a bad length is still reported
+    before = cache.k.clone()
+    ctx.kv_evict(cache, ints(20, 21, 0).cuda(), 20)
+    assert ctx.device_status(reset=True) == BAD_ROW
+    assert torch.equal(cache.k, before)
 
 
 # ---- refusals --------------------------------------------------------------------------------------
@@ -458,6 +463,7 @@ def test_batch_refusals(ctx):
     refuses(INVALID, ctx.attention_batch, bare, q, lens, 4, decay=1.0)
     refuses(INVALID, ctx.attention_batch, cache, q, lens, 4, decay=float("nan"))
     refuses(INVALID, ctx.attention_batch, cache, q, lens, 4, scale=float("inf"))
+    refuses(INVALID, ctx.attention_batch, cache, q, lens, 4, scale=3e38)
     refuses(INVALID, ctx.attention_batch, cache, torch.zeros(B, 3 * hd, device="cuda"), lens, 3)
     refuses(INVALID, ctx.attention_batch, cache, q, lens, 4, ws=torch.zeros(16, dtype=torch.uint8, device="cuda"))
     refuses(INVALID, ctx.kv_evict, bare, lens, 8)
