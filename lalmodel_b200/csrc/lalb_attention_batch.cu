@@ -146,8 +146,21 @@ struct Cfg {
     static constexpr uint32_t kGroup = kRows * HD * 4;
     static constexpr int kSlots = HD == 128 ? 1 : 2;
     static constexpr int kBudget = kRaw ? kStageBudgetRaw : kNS == 2 ? kStageBudget2 : kStageBudget1;
-    static constexpr int kStages = kBudget / (int)kStage < 10 ? kBudget / (int)kStage : 10;
+    // F32 at head_dim 256: two slots of K (64 KB) and two of V's half (32) instead of
+    // three of 64, in which a tile's K had to wait for the V two tiles before (4.5
+    // us a tile)
+    static constexpr bool kTwoRings = kNDV == 2;
+    static constexpr int kStages = kTwoRings ? 4 : kBudget / (int)kStage < 10 ? kBudget / (int)kStage : 10;
     static_assert(kStages >= 2 * kAhead + 1, "V(j) to K(j + kAhead) are held at once");
+    // Stage st = 2 t (K of the CTA's tile t) or 2 t + 1 (its V): its slot, how often
+    // the slot was used before, and the slot's place
+    static __device__ __forceinline__ uint32_t slot(uint32_t st) {
+        return kTwoRings ? 2 * (st & 1) + (st >> 1 & 1) : st % kStages;
+    }
+    static __device__ __forceinline__ uint32_t uses(uint32_t st) { return kTwoRings ? st >> 2 : st / kStages; }
+    static __device__ __forceinline__ uint32_t place(uint32_t slot) {
+        return kTwoRings && slot >= 2 ? 2 * kStage + (slot - 2) * (kStage / 2) : slot * kStage;
+    }
     static_assert(kStages / 2 + 2 <= kSide, "a tile's scales outlive its stages");
     // Narrow heads' tiles come in faster than one warp weighs them (8 sequences
     // of 3001 to 8191 scored f16 rows at head_dim 64: 45 us without, 39 with; F32
@@ -157,7 +170,7 @@ struct Cfg {
     static constexpr bool kFewOk = HD <= 64;
     static constexpr int kSubW = HD < 64 ? HD : 64;                   // columns of a swizzled subtile
     static constexpr uint32_t kSub = kTile * kSubW * 2;               // its bytes
-    static constexpr uint32_t kOffScratch = kStages * kStage;         // 4 KB per softmax warp
+    static constexpr uint32_t kOffScratch = kTwoRings ? 3 * kStage : kStages * kStage;   // 4 KB per softmax warp
     static constexpr uint32_t kOffRaw = kOffScratch + kSoftWarps * 4096;
     static constexpr uint32_t kOffMl = kOffRaw + (kRaw ? kLoadWarps * kSlots * kGroup : 0);
     static constexpr uint32_t kOffSide = kOffMl + 2 * (2 * kM * 8 + 32);   // ml and qmax, of two segments
@@ -668,9 +681,9 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 return true;
             };
             auto finish = [&](const auto &x, int k, int e) {
-                const uint32_t st = k / C::kGroups, g = k % C::kGroups, slot = st % C::kStages, use = st / C::kStages;
+                const uint32_t st = k / C::kGroups, g = k % C::kGroups, slot = C::slot(st), use = C::uses(st);
                 if (use > 0) ok = ok && warp_wait(&empty[slot], (use - 1) & 1u, a.status);
-                x.store(smem + slot * C::kStage, C::kRows * g, pow2(-e), C::kGrid4 && !(st & 1), lane);     // even stages: keys
+                x.store(smem + C::place(slot), C::kRows * g, pow2(-e), C::kGrid4 && !(st & 1), lane);     // even stages: keys
                 // K: the factor that undoes the scaling; V: the exponent
                 if (lane == 0) side[((st >> 1) % kSide) * 16 + (st & 1) * 8 + g] = st & 1 ? (float)e : pow2(e);
                 fence_async();
@@ -742,7 +755,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                 for (int j = s.j0; j < s.j1 && ok; ++j)
 #pragma unroll 1
                     for (int kv = 0; kv < 2 && ok; ++kv, ++st) {
-                        const uint32_t slot = st % C::kStages, use = st / C::kStages;
+                        const uint32_t slot = C::slot(st), use = C::uses(st);
                         if (use > 0 && !wait_bounded(&empty[slot], (use - 1) & 1u, a.status)) {
                             ok = false;
                             break;
@@ -750,14 +763,14 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         mbar_arrive_expect_tx(&full[slot], C::kStage);
 #pragma unroll
                         for (int c = 0; c < HD / C::kSubW; ++c)
-                            tma2d(smem + slot * C::kStage + c * C::kSub, kv ? mv : mk, s.g * HD + c * C::kSubW,
+                            tma2d(smem + C::place(slot) + c * C::kSub, kv ? mv : mk, s.g * HD + c * C::kSubW,
                                   row0 + j * kTile, &full[slot]);
                     }
             }
             // nothing may still be on its way into this CTA's shared memory when it ends
 #pragma unroll 1
             for (uint32_t i = st > (uint32_t)C::kStages ? st - C::kStages : 0; i < st; ++i)
-                wait_bounded(&full[i % C::kStages], (i / C::kStages) & 1u, a.status);
+                wait_bounded(&full[C::slot(i)], C::uses(i) & 1u, a.status);
         }
     } else if (warp == C::kSoftWarps) {
         // ================================ MMA ====================================================
@@ -769,13 +782,13 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         uint32_t tile = 0, segs = 0;        // tiles before the segment: its K(i) is stage 2 (tile + i)
         bool ok = true;
         auto issue_pv = [&](uint32_t t, bool first) -> bool {
-            const uint32_t buf = t % C::kBufs, sv = (2 * t + 1) % C::kStages, use = (2 * t + 1) / C::kStages;
+            const uint32_t buf = t % C::kBufs, sv = C::slot(2 * t + 1), use = C::uses(2 * t + 1);
             if (!warp_wait(&pready[buf], (t / C::kBufs) & 1u, a.status) ||
                 !warp_wait(&full[sv], use & 1u, a.status))
                 return false;
             tc_after();
             const uint32_t stream = C::kNS == 2 ? t & 1u : 0;
-            const uint32_t d = C::kColO + stream * C::kDV, p = C::kColS + buf * kTile, v = ring + sv * C::kStage;
+            const uint32_t d = C::kColO + stream * C::kDV, p = C::kColS + buf * kTile, v = ring + C::place(sv);
             // weights: of 16 scores' 16 columns, 8 hold the high parts, 8 the rest
             auto hi = [&](int kk) { return p + 16 * kk; };
             auto v_off = [&](int kk) { return v + kk * 16 * C::kSubW * 2; };
@@ -803,10 +816,10 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             for (int i = 0; i < n + C::kAhead && ok; ++i) {
                 if (i < n) {
                     const uint32_t t = tile + i, buf = t % C::kBufs;
-                    const uint32_t sk = 2 * t % C::kStages, use = 2 * t / C::kStages;
+                    const uint32_t sk = C::slot(2 * t), use = C::uses(2 * t);
                     if (!(ok = warp_wait(&full[sk], use & 1u, a.status))) break;
                     tc_after();
-                    const uint32_t d = C::kColS + buf * kTile, k = ring + sk * C::kStage;
+                    const uint32_t d = C::kColS + buf * kTile, k = ring + C::place(sk);
                     auto k_off = [&](int kk) {
                         return k + (kk / (C::kSubW / 16)) * C::kSub + (kk % (C::kSubW / 16)) * 32;
                     };
@@ -1192,8 +1205,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         // stale rows behind a sequence's end may hold anything, NaN too,
                         // and 0 x NaN is NaN: the values' tile gets zeros there
                         if (!s.prefix && valid < kTile) {
-                            ok = ok && warp_wait(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
-                            uint8_t *v = smem + (sv % C::kStages) * C::kStage;
+                            ok = ok && warp_wait(&full[C::slot(sv)], C::uses(sv) & 1u, a.status);
+                            uint8_t *v = smem + C::place(C::slot(sv));
                             constexpr int kU = C::kSubW * 2 / 16;
                             const int units = (kTile - valid) * kU;
 #pragma unroll
@@ -1205,7 +1218,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                             fence_async();
                         }
                     } else {
-                        ok = ok && warp_wait(&full[sv % C::kStages], (sv / C::kStages) & 1u, a.status);
+                        ok = ok && warp_wait(&full[C::slot(sv)], C::uses(sv) & 1u, a.status);
                     }
                     if (active && ok) {
                         const uint32_t sc = lanes + C::kColS + buf * kTile;
