@@ -91,7 +91,8 @@ constexpr int kGrid = 148;           // one CTA per SM of a B200 (workspace size
 constexpr int kTile = 64;            // cache rows per tile
 constexpr int kM = 128;              // query rows per unit
 constexpr int kFew = 16;             // units of at most so many rows: a tile's columns are split over the warps
-constexpr int kPad = 3;              // list places a unit takes beside its tiles: what its segment's ends cost
+// list places a unit takes beside its tiles: what its segment's ends cost
+constexpr int kPad16 = 3, kPadF32 = 2;
 constexpr int kLens = 512;           // sequences whose lengths a CTA keeps in shared memory
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (Cfg checks that they outlive the ring)
 // F32: a stream's tiles between two additions of its O to the sum in memory (1, 2,
@@ -196,25 +197,25 @@ struct AbArgs {
     int n_seq, n_head, n_kv, group, max_ctx, prefix, add_weights;
     int m_p, m_o;                // 128-row tiles of a prefix and an own unit's KV head
     int rows_p, rows_o;          // rows kept per partial: query rows of a prefix and an own unit at most
-    int pitch;
+    int pitch, pad;              // score rows' distance; empty list places of a unit
     float c, decay, sign;        // |scale| log2 e, sign of the scale
 };
 
 __host__ __device__ inline int tiles_of(int rows) { return (rows + kTile - 1) / kTile; }
 
-// List places of a unit over n rows: its tiles after kPad empty ones.
-__host__ __device__ inline int places_of(int rows) { return rows > 0 ? kPad + tiles_of(rows) : 0; }
+// List places of a unit over n rows: its tiles after `pad` empty ones.
+__host__ __device__ inline int places_of(int rows, int pad) { return rows > 0 ? pad + tiles_of(rows) : 0; }
 
 // A length outside the cache counts as 0.
 __device__ __forceinline__ int checked_len(const AbArgs &a, int n) { return n < 0 || n > a.max_ctx ? 0 : n; }
 
 // The list: the prefix units' places first, then per sequence its units'.
 // CTA c takes `per` places, the first `rem` CTAs one more.  A segment's ends
-// (Q, the pipeline's fill and drain, the partial) take as long as about three
+// (Q, the pipeline's fill and drain, the partial) take as long as two or three
 // tiles; without empty places for them, CTAs with many short units finish last
 // (64 sequences of up to 1000 rows behind a prefix of 16384, bf16: 69 us, with
-// 3 places 52, with 2 or 4 60 and 54; 30 F32 sequences of up to 1000: 39, 39
-// and 46 with 3, 2 and 4).
+// 3 places 52, with 2 or 4 60 and 54; 30 F32 sequences of up to 1000 rows: 43, 41
+// and 46 with 3, 2 and 4, 50 of up to 100 behind 1000: 35 and 31 with 3 and 2).
 // (The host bounds every index.)
 struct List {
     int tp, total;         // places of the prefix units, all places
@@ -223,7 +224,7 @@ struct List {
     int per, rem;
 
     __device__ __forceinline__ List(const AbArgs &a, int ndv, int own_places) {
-        lt = places_of(a.prefix);
+        lt = places_of(a.prefix, a.pad);
         tp = a.n_kv * a.m_p * ndv * lt;
         units_o = a.n_kv * a.m_o * ndv;
         total = tp + own_places * units_o;
@@ -277,7 +278,7 @@ struct Walk {
                     c0 += np * l.units_o;
                     ++b;
                     n = checked_len(a, b < kLens ? lens_s[b] : __ldcg(a.lens + b));
-                    np = places_of(n);
+                    np = places_of(n, a.pad);
                 }
                 u = (o - c0) / np;
                 p0 = o - c0 - u * np;
@@ -290,8 +291,8 @@ struct Walk {
             }
             const int p1 = min(places, p0 + (end - t));
             t += p1 - p0;
-            s.j0 = max(0, p0 - kPad);
-            s.j1 = p1 - kPad;
+            s.j0 = max(0, p0 - a.pad);
+            s.j1 = p1 - a.pad;
             if (s.j1 <= s.j0) continue;      // empty places only
             const int v = u / NDV;
             s.dv = u - v * NDV;
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         int sum = 0;
 #pragma unroll 1
         for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-            const int n = length(b0 + lane), nt = places_of(checked_len(a, n)), incl = scan(nt);
+            const int n = length(b0 + lane), nt = places_of(checked_len(a, n), a.pad), incl = scan(nt);
             if (blockIdx.x == 0) {
                 if (n < 0 || n > a.max_ctx) atomicOr(a.status, LALB_STATUS_BAD_POSITION);
                 if (b0 + lane < a.n_seq) a.cum[b0 + lane] = sum + incl - nt;
@@ -603,7 +604,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             int run = 0;
 #pragma unroll 1
             for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-                const int n = length(b0 + lane), nt = places_of(checked_len(a, n)), incl = scan(nt);
+                const int n = length(b0 + lane), nt = places_of(checked_len(a, n), a.pad), incl = scan(nt);
                 const uint32_t past = __ballot_sync(0xffffffffu, run + incl > want);
                 if (past) {
                     const int i = __ffs(past) - 1;
@@ -637,7 +638,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     walk.b = *start_b;
     walk.c0 = start[1] * list.units_o;
     walk.n = start[2];
-    walk.np = places_of(walk.n);
+    walk.np = places_of(walk.n, a.pad);
     walk.lens_s = lens_s;
     Seg s;
 
@@ -1441,12 +1442,12 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
         const int up = (g * a.m_p + rp / kM) * C::kNDV + dv, uo = (g * a.m_o + hh / kM) * C::kNDV + dv;
         int np = 0, no = 0, cp = 0, co = 0;
         if (l.lt > 0) {
-            cp = l.owner(up * l.lt + kPad);
+            cp = l.owner(up * l.lt + a.pad);
             np = l.owner(up * l.lt + l.lt - 1) - cp + 1;
         }
         if (places > 0) {
             const int to = l.tp + cum * l.units_o + uo * places;
-            co = l.owner(to + kPad);
+            co = l.owner(to + a.pad);
             no = l.owner(to + places - 1) - co + 1;
         }
         const size_t r0p = (size_t)(cp + up) * a.rows_p + rp % kM;
@@ -1536,8 +1537,8 @@ int ab_shape(const lalb_kv_batch *c, const lalb_attn_batch *p) {
         return LALB_ERR_UNSUPPORTED;
     // places of the list at most, and query rows: 31-bit indices
     const long long mp = (c->n_seq * group + kM - 1) / kM, mo = (group + kM - 1) / kM;
-    const long long tiles = 2ll * c->n_kv_head * (mp * places_of(p->prefix_len) +
-                                                  mo * c->n_seq * (long long)places_of(c->max_ctx));
+    const long long tiles = 2ll * c->n_kv_head * (mp * places_of(p->prefix_len, kPad16) +
+                                                  mo * c->n_seq * (long long)places_of(c->max_ctx, kPad16));
     if (tiles > (1ll << 30) || c->n_seq * group > (1ll << 30)) return LALB_ERR_UNSUPPORTED;
     return LALB_OK;
 }
@@ -1563,6 +1564,7 @@ void make_plan(const lalb_kv_batch *c, const lalb_attn_batch *p, Plan *pl) {
     a.rows_p = std::min(kM, a.n_seq * a.group);
     a.rows_o = std::min(kM, a.group);
     a.pitch = tiles_of(a.max_ctx) * kTile;
+    a.pad = c->dtype == LALB_DT_F32 ? kPadF32 : kPad16;
     const int hd = c->head_dim, dv = hd / ndv;
     // a segment's slot is its CTA's number plus its unit's
     const size_t sp = a.prefix ? (size_t)kGrid + (size_t)a.n_kv * a.m_p * ndv : 0;
