@@ -361,11 +361,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
         : "memory");
 }
 
-// The value every lane holds anyway, known to the compiler as one for the
-// warp: the MMA operands derived from it are computed in uniform registers
-// instead of moved there one by one for each instruction.
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-
 // A warpgroup's registers from here on (0: as launched).  In the role's own
 // branch: where roles meet again the compiler keeps to the smaller share.
 template <int N, bool INC>
