@@ -66,9 +66,9 @@
 //     segments cost 3 us each;
 //   16 sequences, 4093 + 1..700 F32 rows: 31 us, floor 6; one tile takes its
 //     CTA 2 us, most of it in the loaders' splitting and the softmax's waits;
-//   5 sequences, 333 + 100..2000 F32 rows at head_dim 256: 47 us, floor 7; the
-//     ring holds three stages of 64 KB, so that a tile's keys are split only
-//     after the values before the last are used: 4.5 us a tile;
+//   5 sequences, 333 + 100..2000 F32 rows at head_dim 256: 44 us, floor 7; one
+//     softmax stream for half of the value columns, 64 KB of keys split for each,
+//     and 8 us a segment to bring Q's two parts into TMEM;
 //   8 sequences, 3001..8191 f16 rows, 16 heads on 8 of 64: 40 us, floor 14;
 //   one sequence of 812 F32 rows: 16 us, of which each CTA's single tile takes 8
 //     from launch to partial, all latency: lengths, Q, rows, S, weights, PV in turn.
