@@ -213,7 +213,8 @@ typedef struct {
  * cache stores nothing and raises status bit 2 (lalb_device_status).  No two
  * tokens of a call may have the same slot.  slots NULL: only q is rotated.
  * A negative position turns back, so that a rotation's gradient is the
- * rotation by the negated positions.  qkv rows and q_out 16-byte aligned. */
+ * rotation by the negated positions.  qkv rows and q_out 16-byte aligned;
+ * qkv overlaps neither q_out nor the cache. */
 LALB_API int lalb_rope_append(lalb_ctx *ctx, const lalb_rope *rope, const lalb_kv_batch *cache,
                               int n_head, const void *qkv, int qkv_dtype, long long qkv_stride,
                               int T, const int32_t *positions, const int32_t *slots, void *q_out,
@@ -235,8 +236,8 @@ LALB_API int lalb_rope_append(lalb_ctx *ctx, const lalb_rope *rope, const lalb_k
  * F16 and BF16: weights enter as two parts of that type.  A
  * length outside its range counts as 0 and raises status bit 2.  ws: from
  * lalb_attention_batch_ws_bytes, 256-byte aligned, nothing kept between
- * calls; calls that may overlap need one each.  The result does not depend
- * on scheduling. */
+ * calls; calls that may overlap need one each.  out may be q's own rows.  The
+ * result does not depend on scheduling. */
 typedef struct {
     int n_head;
     float scale;
@@ -260,9 +261,10 @@ LALB_API int lalb_attention_batch(lalb_ctx *ctx, const lalb_kv_batch *cache,
  * copied.  Afterwards lens[b] = keep and row_weight of rows keep..old
  * length-1 is 0; the rest of those rows, and all rows behind them, are left as
  * they were.  Sequences of at most `keep` rows are left as they are; a length
- * outside [0, max_ctx] raises status bit 2 and is left too.  The cache needs row_pos and row_weight.
- * 1 <= keep <= max_ctx, n_sink + n_recent <= keep.  ws: from
- * lalb_kv_evict_ws_bytes, 256-byte aligned. */
+ * outside [0, max_ctx] raises status bit 2 and is left too.  The cache needs
+ * row_pos and row_weight.  1 <= keep <= max_ctx, n_sink + n_recent <= keep.
+ * ws: from lalb_kv_evict_ws_bytes, 256-byte aligned; nothing is kept in it
+ * between calls, and calls that may overlap need one each. */
 LALB_API int lalb_kv_evict_ws_bytes(const lalb_kv_batch *cache, int keep, size_t *bytes);
 LALB_API int lalb_kv_evict(lalb_ctx *ctx, const lalb_kv_batch *cache, int32_t *lens, int keep,
                            int n_sink, int n_recent, void *ws, lalb_stream stream);

@@ -427,6 +427,54 @@ def test_kv_evict_bad_length_is_reported_and_left(ctx):
     assert torch.equal(cache.k, before)
 
 
+def test_two_graphs_share_a_workspace(ctx):
+    """A step of attention whose output replaces its queries, and an eviction,
+    each in a graph, replayed in turn over one workspace."""
+    nh, nk, hd, L, C, B, keep = 6, 2, 64, 130, 200, 3, 90
+    k, v = rand(1, B, C, nk * hd), rand(2, B, C, nk * hd)
+    pk, pv = rand(3, L, nk * hd), rand(4, L, nk * hd)
+    pos = torch.arange(C, dtype=torch.int32).expand(B, nk, C).contiguous()
+    cache = lb.KVBatch(k.cuda(), v.cuda(), nk, pos.cuda(), torch.zeros(B, nk, C, device="cuda"))
+    q, lens, pkd, pvd = torch.zeros(B, nh * hd, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda"), \
+        pk.cuda(), pv.cuda()
+    ws = max(ctx.attention_batch_ws(cache, nh, L, True), ctx.kv_evict_ws(cache, keep), key=lambda t: t.numel())
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        calls = (lambda: ctx.attention_batch(cache, q, lens, nh, pkd, pvd, decay=1.0, ws=ws, out=q),
+                 lambda: ctx.kv_evict(cache, lens, keep, n_sink=2, n_recent=5, ws=ws))
+        graphs = []
+        for call in calls:
+            call()
+            s.synchronize()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=s):
+                call()
+        for i, n in enumerate(([200, 90, 120], [91, 0, 200], [1, 150, 89])):
+            qh = rand(50 + i, B, nh * hd)
+            q.copy_(qh)
+            lens.copy_(ints(*n))
+            before = (cache.k.cpu(), cache.v.cpu(), cache.row_weight.cpu())
+            graphs[0].replay()
+            s.synchronize()
+            ref, w, mag, top = R.attention(qh, *before[:2], ints(*n), nh, nk, pk, pv)
+            within(q, ref, attn_tol(ref, mag, top, torch.float32, L + C))
+            got = cache.row_weight.cpu()
+            step = score_step(top).view(B, nk, -1).amax(-1)[:, :, None]
+            within(got, before[2].double() + w,                 # run_attention's bound
+                   w * (2 * step + 2.0 ** -21 + (64 + (L + C) / 64 + 8) * 2.0 ** -24)
+                   + 3 * 2.0 ** -24 * (before[2].double() + w))
+            rl, rp, rw, moves = R.evict(ints(*n), cache.row_pos.cpu(), got, keep, 2, 5)
+            graphs[1].replay()
+            s.synchronize()
+            assert torch.equal(lens.cpu(), rl) and torch.equal(cache.row_pos.cpu(), rp)
+            assert torch.equal(cache.row_weight.cpu(), rw)
+            assert torch.equal(cache.k.cpu(), R.apply_moves(before[0], moves, nk))
+            assert torch.equal(cache.v.cpu(), R.apply_moves(before[1], moves, nk))
+    for g in graphs:
+        g.reset()
+
+
 # ---- refusals --------------------------------------------------------------------------------------
 def test_batch_refusals(ctx):
     hd, nk, B, C = 64, 2, 2, 16
