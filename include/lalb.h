@@ -232,7 +232,9 @@ LALB_API int lalb_rope_append(lalb_ctx *ctx, const lalb_rope *rope, const lalb_k
  * read); the prefix rows' weights are not kept.  q, the caches and out have
  * the cache's type; q row b starts at q + b*q_stride elements.  F32: keys,
  * queries, values and weights enter the tensor cores as two fp16 parts (22
- * bits) under powers of two shared by 16 rows, products are summed in fp32.
+ * bits), a query row under a power of two of its own, keys and values under
+ * one shared by 16 neighbouring rows (8 at head_dim 256); products are summed
+ * in fp32.
  * F16 and BF16: weights enter as two parts of that type.  A
  * length outside its range counts as 0 and raises status bit 2.  ws: from
  * lalb_attention_batch_ws_bytes, 256-byte aligned, nothing kept between

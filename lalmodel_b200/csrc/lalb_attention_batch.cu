@@ -174,7 +174,8 @@ struct Cfg {
     static constexpr uint32_t kOffScratch = kTwoRings ? 3 * kStage : kStages * kStage;   // 4 KB per softmax warp
     static constexpr uint32_t kOffRaw = kOffScratch + kSoftWarps * 4096;
     static constexpr uint32_t kOffMl = kOffRaw + (kRaw ? kLoadWarps * kSlots * kGroup : 0);
-    static constexpr uint32_t kOffSide = kOffMl + 2 * (2 * kM * 8 + 32);   // ml and qmax, of two segments
+    // (m, l) and, F32, each query row's largest |q|: per stream and row, of two segments
+    static constexpr uint32_t kOffSide = kOffMl + 2 * 2 * kM * (kF32 ? 12 : 8);
     static constexpr uint32_t kOffLens = kOffSide + kSide * 16 * 4;
     static constexpr uint32_t kOffBar = kOffLens + kLens * 4;
     static constexpr uint32_t kSmem = 1024 + kOffBar + 512;
@@ -858,7 +859,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         // Two of each, taken in turn: a warpgroup without a tile in a segment may
         // be at the next boundary while the other still reads this one's.
         float2 *ml = reinterpret_cast<float2 *>(smem + C::kOffMl);    // [stream][row]: (m, l)
-        float *qmax = reinterpret_cast<float *>(ml + 2 * 2 * kM);     // F32: largest |q| of a warp's rows and columns
+        float *qmax = reinterpret_cast<float *>(ml + 2 * 2 * kM);     // F32: [warpgroup][row], largest |q| of its columns
         uint32_t turn = 0;
         uint32_t tile = 0;                      // before the segment
         uint32_t pv0 = 0, pv1 = 0;              // products of each stream so far
@@ -903,13 +904,13 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     while (h >= a.group) h -= a.group, ++b;
             }
         };
-        // F32: the largest |q| of the warp's rows in a batch
-        auto q_top = [&](const uint4 (&v)[kBatch * kIt], float top) {
+        // F32: the largest |q| in a batch, this lane's columns of its kIt rows
+        auto q_top = [&](const uint4 (&v)[kBatch * kIt], float (&top)[kIt]) {
 #pragma unroll
             for (int i = 0; i < kBatch * kIt; ++i)
-                top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(v[i].x)), fabsf(__uint_as_float(v[i].y))),
-                                       fmaxf(fabsf(__uint_as_float(v[i].z)), fabsf(__uint_as_float(v[i].w)))));
-            return top;
+                top[i % kIt] =
+                    fmaxf(top[i % kIt], fmaxf(fmaxf(fabsf(__uint_as_float(v[i].x)), fabsf(__uint_as_float(v[i].y))),
+                                              fmaxf(fabsf(__uint_as_float(v[i].z)), fabsf(__uint_as_float(v[i].w)))));
         };
         auto q_store = [&](int c0, const uint4 (&v)[kBatch * kIt], float qs) {
 #pragma unroll
@@ -950,26 +951,38 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
         auto q_share = [&](const Seg &g) {
             if constexpr (C::kF32) {
                 if (first_row(g) >= g.rows || q_idle) return;
-                float top = q_top(qv, 0.0f);
+                float top[kIt] = {};
+                q_top(qv, top);
 #pragma unroll 1
                 for (int c = kBatch; c < kChunks; c += kBatch) {
                     uint4 v[kBatch * kIt];
                     q_load(g, c, v);
-                    top = q_top(v, top);
+                    q_top(v, top);
                 }
-                top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                if (lane == 0) qmax[turn * 8 + warp] = top;
+                // over the kLpr lanes of a row, as many as a lane has rows: at each
+                // step a lane hands on one half of its rows and keeps the other, at
+                // the end it has row kRpi * lu + lr
+                static_assert(kLpr == kIt, "a lane ends with one row");
+#pragma unroll
+                for (int o = kLpr / 2; o > 0; o >>= 1)
+#pragma unroll
+                    for (int i = 0; i < o; ++i) {
+                        const bool up = lu & o;
+                        const float away = up ? top[i] : top[i + o];
+                        top[i] = fmaxf(up ? top[i + o] : top[i], __shfl_xor_sync(0xffffffffu, away, o));
+                    }
+                qmax[(turn * 2 + wg) * kM + quarter * 32 + kRpi * lu + lr] = top[0];
             }
         };
-        // .. and after it: Q written (F32: under the power of two of its 32 rows), the
-        // rows' score factor returned
+        // .. and after it: Q written (F32: each row under its own power of two, so that
+        // no row's size, not even an infinity, reaches the rows of other heads and
+        // sequences), the row's score factor returned
         auto q_finish = [&](const Seg &g) -> float {
             float qs = a.sign, cq = a.c;
             if (first_row(g) < g.rows) {
                 if constexpr (C::kF32) {
-                    const float *qm = qmax + turn * 8 + quarter;
-                    const float top = C::kNS == 2 && HD > 32 ? fmaxf(qm[0], qm[4]) : qm[0];
-                    const int e = part_exponent(top);
+                    const float *qm = qmax + turn * 2 * kM + row;
+                    const int e = part_exponent(C::kNS == 2 && HD > 32 ? fmaxf(qm[0], qm[kM]) : qm[0]);
                     qs = a.sign * pow2(-e);
                     cq = a.c * pow2(e);
                 }

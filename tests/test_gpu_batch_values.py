@@ -1,0 +1,92 @@
+"""lalb_attention_batch on values of very different sizes and on values that
+are not finite: what one head, sequence or row holds must not reach another."""
+import math
+
+import pytest
+import torch
+
+import _batch_ref as R
+import lalmodel_b200 as lb
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+# F32, ||error|| / ||out|| of one head's row, for scores of order 1 (|s| <= 4
+# over a thousand rows).  The tensor cores cut each addition off by 2^-24 of
+# the running sum on average.  Scores: 16 large additions at most (head_dim
+# 256), sums that grow from 0 to s, |s| 2 in the root mean square of the rows
+# that matter: 16 * 2^-24 * 2 = 1.9e-6.  Outputs: 12 additions a tile, four
+# tiles to a sum that grows from 0: 48 / 2 * 2^-24 = 1.4e-6; rounding of
+# streams, partials and 22-bit parts: 10 * 2^-24 = 0.6e-6.
+F32_NORM = 4e-6
+
+
+def rand(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+class Case:
+    """A batch with a prefix: sequences and heads of a small attention call."""
+
+    def __init__(self, dtype, B, nh, nk, hd, L, lens, seed):
+        dt = DT[dtype]
+        self.B, self.nh, self.nk, self.hd, self.lens = B, nh, nk, hd, ints(*lens)
+        C = max(lens) + 3
+        self.q = rand(seed, B, nh * hd, dtype=dt)
+        self.k, self.v = rand(seed + 1, B, C, nk * hd, dtype=dt), rand(seed + 2, B, C, nk * hd, dtype=dt)
+        self.pk = rand(seed + 3, L, nk * hd, dtype=dt) if L else None
+        self.pv = rand(seed + 4, L, nk * hd, dtype=dt) if L else None
+        self.w = None
+
+    def run(self, ctx, decay=None):
+        w = None if decay is None else torch.zeros(self.B, self.nk, self.k.shape[1], device="cuda")
+        cache = lb.KVBatch(self.k.cuda(), self.v.cuda(), self.nk, row_weight=w)
+        out = ctx.attention_batch(cache, self.q.cuda(), self.lens.cuda(), self.nh,
+                                  None if self.pk is None else self.pk.cuda(),
+                                  None if self.pv is None else self.pv.cuda(), decay=decay)
+        self.w = None if w is None else w.cpu()
+        return out.cpu().view(self.B, self.nh, self.hd)
+
+    def exact(self):
+        out = R.attention(self.q, self.k, self.v, self.lens, self.nh, self.nk, self.pk, self.pv)[0]
+        return out.view(self.B, self.nh, self.hd)
+
+
+def head_errors(got, ref):
+    """||error|| / ||ref|| of each (sequence, head)."""
+    return (got.double() - ref).norm(dim=-1) / ref.norm(dim=-1)
+
+
+# (B, nh, nk, L, lens): query rows of a prefix unit above and up to 16
+MANY, FEW = (5, 8, 2, 333, (200, 70, 0, 64, 1)), (3, 4, 2, 70, (40, 130, 9))
+
+
+@pytest.mark.parametrize("shape", [MANY, FEW])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_f32_one_sequences_queries_leave_the_others(ctx, hd, shape):
+    """One sequence's queries 2^12, 2^30 or 1e30 times larger, or infinite; the
+    others' outputs stay as exact as they are without."""
+    B, nh, nk, L, lens = shape
+    for big in (2.0 ** 12, 2.0 ** 30, 1e30, float("inf")):
+        c = Case("f32", B, nh, nk, hd, L, lens, seed=hd + B)
+        ref = c.exact()
+        c.q[1] *= big
+        others = [b for b in range(B) if b != 1]
+        err = head_errors(c.run(ctx), ref)[others]
+        assert float(err.max()) <= F32_NORM, (big, err)
+    assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_f32_heads_of_different_size(ctx, hd):
+    """Every other head's queries 2^10 times larger: the heads beside them, in
+    the prefix's units and in each sequence's own, stay as exact."""
+    c = Case("f32", 4, 8, 2, hd, 150, (90, 0, 33, 128), seed=hd)
+    c.q.view(c.B, c.nh, hd)[:, ::2] *= 2.0 ** 10
+    err = head_errors(c.run(ctx), c.exact())[:, 1::2]
+    assert float(err.max()) <= F32_NORM, err
