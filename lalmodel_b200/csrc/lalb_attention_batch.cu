@@ -43,17 +43,19 @@
 //            enter PV as two parts, so that they are not rounded to the
 //            cache's type (one part: 1.4 times the output error).
 //
-// F32: x = hi + lo in fp16 (22 bits).  The rows of a tile that a loader warp
-// splits at a time share a power of two that puts their largest |x| in
-// [2^14, 2^15); K's goes into the scores' factor, V's exponent e into the
+// F32: x = hi + lo in fp16, hi x rounded and lo the rest: 22 bits of every
+// element above 2^-17 of the largest that shares its scale.  A query row has a
+// scale of its own; the rows of a tile that a loader warp splits at a time share
+// a power of two that puts their largest |x| in [2^14, 2^15); K's goes into the scores' factor, V's exponent e into the
 // weights' exponent: p' = 2^(x + e - m), v' = v 2^-e, so that p' keeps its
 // precision whatever the values' range, and l takes p' 2^-e.  m is an integer:
 // x + (e - m) then rounds once, at the size of the exponent that matters.
 //
 // The tensor cores cut every addition to an accumulator off towards zero.  In S
-// the small products go first, while the sum is small (at head_dim 256 with the
-// product of the two rests, and with high parts whose products add up exactly:
-// split_grid).  O, 12 additions a tile, came out 1e-5 too
+// the small products go first, while the sum is small.  (High parts on one grid,
+// whose products add up exactly, took the output error at head_dim 256 from 1.3
+// to 0.8e-6 of the whole, but left an element 2^-12 of the largest only 11 bits:
+// 2e-4 behind keys 2^10 times larger.)  O, 12 additions a tile, came out 1e-5 too
 // small after 64 tiles of a stream: F32 adds it to a sum in global memory,
 // rounded to nearest, every kFlush tiles and starts it again from zero.
 //
@@ -136,10 +138,6 @@ struct Cfg {
     static_assert(kSoftRegs == 0 || kSoftRegs * kSoftWarps + kOtherRegs * kOtherWarps <=
                                         kEven * (kSoftWarps + kOtherWarps),
                   "the split is no more than the block was launched with");
-    // F32 keys and queries on a grid, all four products: at head_dim 256 the
-    // output error goes from 2.0 to 0.9e-6 of the whole; at 128 it would go from
-    // 1.1 to 0.9 (1024 rows) for 2 of 33 us (16 sequences behind 4093 rows)
-    static constexpr bool kGrid4 = HD == 256;
     static constexpr uint32_t kStage = kTile * HD * (kF32 ? 4 : 2);
     // F32 rows come in raw, a group at a time, into a slot of the loader warp
     // that splits them (head_dim 256 has no room: plain loads)
@@ -400,7 +398,7 @@ __device__ __forceinline__ uint32_t split2(float2 x, uint32_t &lo) {
     return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);   // bf16: the upper halves
 }
 
-// F32's weights and values: the high part is x rounded to fp16, so that the
+// F32: the high part is x rounded to fp16, so that the
 // rests have either sign and the product of two rests, which is left out, is 0
 // on average and not 2^-22 of the whole.
 __device__ __forceinline__ uint32_t split_rn(float2 x, uint32_t &lo) {
@@ -409,18 +407,6 @@ __device__ __forceinline__ uint32_t split_rn(float2 x, uint32_t &lo) {
     const float2 r = __fadd2_rn(x, make_float2(-h.x, -h.y));
     lo = pack2<__half>(r.x, r.y);
     return hi;
-}
-
-// Keys and queries, in (-2^15, 2^15): the high part is x rounded to a multiple
-// of 16 (11 bits), the rest is within 8 and so held to 2^-9.  High parts on one
-// grid make the sums of their products integers below 2^24 in all but the
-// largest scores, which the tensor cores add without cutting anything off.
-__device__ __forceinline__ uint32_t split_grid(float2 x, uint32_t &lo) {
-    const float2 m = make_float2(201326592.0f, 201326592.0f);    // 1.5 x 2^27: its unit is 16
-    const float2 t = __fadd2_rn(x, m), h = __fadd2_rn(t, make_float2(-m.x, -m.y));
-    const float2 r = __fadd2_rn(x, make_float2(-h.x, -h.y));
-    lo = pack2<__half>(r.x, r.y);
-    return pack2<__half>(h.x, h.y);
 }
 
 // Exponent e, 2^e the power of two that v 2^-e puts |v| <= amax below 2^15
@@ -494,7 +480,7 @@ struct RowLoad {
         const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         return part_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
     }
-    __device__ __forceinline__ void store(uint8_t *stage, int r0, float scale, bool grid, int lane) const {
+    __device__ __forceinline__ void store(uint8_t *stage, int r0, float scale, int lane) const {
         constexpr int W = COLS < 64 ? COLS : 64;
         constexpr uint32_t kLo = kTile * COLS * 2;
         const int rr = lane / kLanes, cc = (lane % kLanes) * 4;
@@ -503,13 +489,8 @@ struct RowLoad {
             const int r = r0 + i / kVec * kPer + rr, c = cc + (i % kVec) * 4 * kLanes;
             uint2 hi, lo;
             const float2 a = make_float2(x[i].x * scale, x[i].y * scale), b = make_float2(x[i].z * scale, x[i].w * scale);
-            if (grid) {
-                hi.x = split_grid(a, lo.x);
-                hi.y = split_grid(b, lo.y);
-            } else {
-                hi.x = split_rn(a, lo.x);
-                hi.y = split_rn(b, lo.y);
-            }
+            hi.x = split_rn(a, lo.x);
+            hi.y = split_rn(b, lo.y);
             const int unit = (c % W) >> 3;
             const int sw = W == 64 ? unit ^ (r & 7) : unit ^ ((r >> 1) & 3);
             const uint32_t off = (uint32_t)(c / W) * (kTile * W * 2) + r * (W * 2) + sw * 16 + (c & 4) * 2;
@@ -680,7 +661,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
             auto finish = [&](const auto &x, int k, int e) {
                 const uint32_t st = k / C::kGroups, g = k % C::kGroups, slot = C::slot(st), use = C::uses(st);
                 if (use > 0) ok = ok && warp_wait(&empty[slot], (use - 1) & 1u, a.status);
-                x.store(smem + C::place(slot), C::kRows * g, pow2(-e), C::kGrid4 && !(st & 1), lane);     // even stages: keys
+                x.store(smem + C::place(slot), C::kRows * g, pow2(-e), lane);
                 // K: the factor that undoes the scaling; V: the exponent
                 if (lane == 0) side[((st >> 1) % kSide) * 16 + (st & 1) * 8 + g] = st & 1 ? (float)e : pow2(e);
                 fence_async();
@@ -821,16 +802,11 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                         return k + (kk / (C::kSubW / 16)) * C::kSub + (kk % (C::kSubW / 16)) * 32;
                     };
                     // The tensor cores cut each sum off towards zero at its own size: the
-                    // small products go first, while the sum is small (at head_dim 256,
-                    // in the middle of the large ones: 3x the output error).
+                    // small products go first, while the sum is small.
                     if constexpr (C::kF32) {
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
-                            if constexpr (C::kGrid4)
-                                mma_f16_ta(d, C::kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS,
-                                           kk ? 1u : 0u);
-                            mma_f16_ta(d, C::kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS,
-                                       kk || C::kGrid4 ? 1u : 0u);
+                            mma_f16_ta(d, C::kColQ + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk) + kLoK), kIdS, kk ? 1u : 0u);
                             mma_f16_ta(d, C::kColQ + HD / 2 + 8 * kk, kmajor_desc<C::kSubW>(k_off(kk)), kIdS, 1u);
                         }
                     }
@@ -928,8 +904,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     if constexpr (C::kF32) {
                         const float2 a0 = make_float2(__uint_as_float(x.x) * qs, __uint_as_float(x.y) * qs);
                         const float2 a1 = make_float2(__uint_as_float(x.z) * qs, __uint_as_float(x.w) * qs);
-                        hi[2 * u] = C::kGrid4 ? split_grid(a0, lo[2 * u]) : split_rn(a0, lo[2 * u]);
-                        hi[2 * u + 1] = C::kGrid4 ? split_grid(a1, lo[2 * u + 1]) : split_rn(a1, lo[2 * u + 1]);
+                        hi[2 * u] = split_rn(a0, lo[2 * u]);
+                        hi[2 * u + 1] = split_rn(a1, lo[2 * u + 1]);
                     } else {
                         // a negative scale turns the queries' signs
                         const uint32_t f = qs < 0.0f ? 0x80008000u : 0u;

@@ -90,3 +90,23 @@ def test_f32_heads_of_different_size(ctx, hd):
     c.q.view(c.B, c.nh, hd)[:, ::2] *= 2.0 ** 10
     err = head_errors(c.run(ctx), c.exact())[:, 1::2]
     assert float(err.max()) <= F32_NORM, err
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("factor", [64.0, 1024.0])
+def test_f32_outlier_keys_and_channels(ctx, hd, factor):
+    """One key in eight many times larger, pointing away from the queries (it
+    takes no weight); then one channel of all keys larger and of all queries
+    smaller.  Either way the scores that matter are those without."""
+    c = Case("f32", 4, 8, 2, hd, 150, (90, 3, 33, 250), seed=hd + 1)
+    c.q = c.q.abs() * 0.5
+    for k in (c.pk, c.k.view(-1, 2 * hd)):
+        k[::8] = -factor * k[::8].abs()
+    err = head_errors(c.run(ctx), c.exact())
+    assert float(err.max()) <= F32_NORM, err
+    c = Case("f32", 4, 8, 2, hd, 150, (90, 3, 33, 250), seed=hd + 2)
+    c.q.view(-1, hd)[:, 5] /= factor
+    for k in (c.pk, c.k):
+        k.view(-1, hd)[:, 5] *= factor
+    err = head_errors(c.run(ctx), c.exact())
+    assert float(err.max()) <= F32_NORM, err
