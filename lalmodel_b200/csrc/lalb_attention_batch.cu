@@ -1029,7 +1029,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     if (active && (k ? cnt1 : cnt0) > kFlush) flush(k, false);
                 }
             }
-            ml[turn * 2 * kM + wg * kM + row] = make_float2(had && any ? mref : -INFINITY, l);
+            // (l is NaN where a score was, and says so even if all of them were)
+            ml[turn * 2 * kM + wg * kM + row] = make_float2(had && (any || l != l) ? mref : -INFINITY, l);
             if (nhave) q_share(nx);
             tc_before();
             soft_bar();

@@ -110,3 +110,59 @@ def test_f32_outlier_keys_and_channels(ctx, hd, factor):
         k.view(-1, hd)[:, 5] *= factor
     err = head_errors(c.run(ctx), c.exact())
     assert float(err.max()) <= F32_NORM, err
+
+
+def check_heads(got, ref, bad, dtype):
+    """Heads in `bad` [B][nh] are NaN throughout, the others as exact as ever:
+    F32 by F32_NORM, 16 bits by one rounding of every element."""
+    assert bool(torch.isnan(got[bad]).all())
+    err = head_errors(got, ref)[~bad]
+    tol = F32_NORM if dtype == "f32" else torch.finfo(DT[dtype]).eps / 2
+    assert bool((err <= tol).all()), err
+
+
+ALONE = (3, 4, 2, 0, (65, 1, 130))       # no prefix
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [MANY, FEW, ALONE])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_nan_query_stays_in_its_head(ctx, dtype, hd, shape):
+    B, nh, nk, L, lens = shape
+    c = Case(dtype, B, nh, nk, hd, L, lens, seed=hd + 10)
+    ref, bad = c.exact(), torch.zeros(B, nh, dtype=torch.bool)
+    for b, h in ((0, 1), (B - 1, nh - 1)):
+        c.q.view(B, nh, hd)[b, h, hd // 2 + b] = float("nan")
+        bad[b, h] = True
+    check_heads(c.run(ctx, decay=0.0), ref, bad, dtype)
+    # the weights that such a head adds to are NaN, all others numbers
+    group = bad.view(B, nk, nh // nk).any(-1)
+    for b in range(B):
+        assert torch.equal(torch.isnan(c.w[b, :, :lens[b]]).all(-1), group[b] | (torch.tensor(lens[b]) == 0))
+        assert bool(torch.isfinite(c.w[b][~group[b]]).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [MANY, FEW, ALONE])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_nan_key_reaches_the_heads_that_read_it(ctx, dtype, hd, shape):
+    """A NaN in a row's key, the only row of a sequence and the ends of tiles
+    among them: every head that reads it is NaN, and no other."""
+    B, nh, nk, L, lens = shape
+    group = nh // nk
+    for b in range(B):
+        for j in sorted({0, 63, 64, lens[b] - 1}):
+            if not 0 <= j < lens[b]:
+                continue
+            c = Case(dtype, B, nh, nk, hd, L, lens, seed=hd + 11)
+            ref, bad = c.exact(), torch.zeros(B, nh, dtype=torch.bool)
+            c.k[b, j, (nk - 1) * hd + 3] = float("nan")
+            bad[b, (nk - 1) * group:] = True
+            check_heads(c.run(ctx), ref, bad, dtype)
+    if L:
+        c = Case(dtype, B, nh, nk, hd, L, lens, seed=hd + 12)
+        ref, bad = c.exact(), torch.zeros(B, nh, dtype=torch.bool)
+        c.pk[L - 1, 0] = float("nan")
+        bad[:, :group] = True
+        check_heads(c.run(ctx), ref, bad, dtype)
+    assert ctx.device_status() == 0
