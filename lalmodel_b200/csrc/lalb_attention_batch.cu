@@ -470,15 +470,17 @@ struct RowLoad {
                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
     }
-    // The rows' common exponent.
+    // The rows' common exponent: that of their largest finite |x|, so that an
+    // infinity spoils its own products only.  2 x bits + 2^24 drops the sign, and
+    // infinities and NaNs wrap around to less than any other value.
     __device__ __forceinline__ int exponent() const {
-        float m4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t m4[4] = {0, 0, 0, 0};
+        auto key = [](float v) { return 2 * __float_as_uint(v) + (1u << 24); };
 #pragma unroll
         for (int i = 0; i < kN; ++i)
-            m4[i & 3] = fmaxf(m4[i & 3],
-                              fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
-        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        return part_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+            m4[i & 3] = max(m4[i & 3], max(max(key(x[i].x), key(x[i].y)), max(key(x[i].z), key(x[i].w))));
+        const uint32_t m = __reduce_max_sync(0xffffffffu, max(max(m4[0], m4[1]), max(m4[2], m4[3])));
+        return part_exponent(__uint_as_float((max(m, 1u << 24) - (1u << 24)) >> 1));
     }
     __device__ __forceinline__ void store(uint8_t *stage, int r0, float scale, int lane) const {
         constexpr int W = COLS < 64 ? COLS : 64;

@@ -166,3 +166,48 @@ def test_nan_key_reaches_the_heads_that_read_it(ctx, dtype, hd, shape):
         bad[:, :group] = True
         check_heads(c.run(ctx), ref, bad, dtype)
     assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [MANY, FEW, ALONE])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("what", ["inf", "-inf", "nan"])
+def test_value_that_is_not_finite_stays_in_its_column(ctx, dtype, hd, shape, what):
+    B, nh, nk, L, lens = shape
+    group, col, bad = nh // nk, 7, float(what)
+    rest = torch.ones(hd, dtype=torch.bool)
+    rest[col] = False
+    tol = F32_NORM if dtype == "f32" else torch.finfo(DT[dtype]).eps / 2
+    for where in ("own", "prefix") if L else ("own",):
+        c = Case(dtype, B, nh, nk, hd, L, lens, seed=hd + 13)
+        ref = c.exact()
+        spoiled = torch.zeros(B, nh, dtype=torch.bool)
+        if where == "own":
+            for b, j in ((0, lens[0] - 1), (1, 0)):
+                c.v[b, j, (nk - 1) * hd + col] = bad
+                spoiled[b, (nk - 1) * group:] = True
+        else:
+            c.pv[L // 2, col] = bad
+            spoiled[:, :group] = True
+        got = c.run(ctx)
+        assert not bool(torch.isfinite(got[spoiled][:, col]).any())
+        assert bool((head_errors(got[..., rest], ref[..., rest]) <= tol).all())
+        assert bool((head_errors(got, ref)[~spoiled] <= tol).all())
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_infinite_keys(ctx, hd):
+    """F32: the heads that read one are NaN, the others as exact as without.
+    16 bits: a score of -inf is a weight of 0."""
+    for dtype in ("f32", "f16", "bf16"):
+        B, nh, nk, L, lens = MANY
+        c = Case(dtype, B, nh, nk, hd, L, lens, seed=hd + 14)
+        c.q.view(B, nh, hd)[..., 2] = 0.5
+        bad = torch.zeros(B, nh, dtype=torch.bool)
+        ref = c.exact()
+        for b, j in ((0, 199), (1, 0)):
+            c.k[b, j, 2] = -float("inf")
+            bad[b, :nh // nk] = True
+        if dtype != "f32":
+            ref, bad = c.exact(), torch.zeros_like(bad)
+        check_heads(c.run(ctx), ref, bad, dtype)
