@@ -1484,7 +1484,8 @@ __global__ void __launch_bounds__(32 * kCombWarps) attention_combine_kernel(cons
                 }
             }
         }
-        const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;   // no rows: 0 (a NaN stays one)
+        // no rows: 0; rows whose scores are all -inf: 0 / 0, as NaN as a NaN among them
+        const float inv = np + no > 0 ? 1.0f / L : 0.0f;
         if (out) {
             T *o = static_cast<T *>(a.out) + ((size_t)b * a.n_head + (size_t)g * a.group + hh) * HD + dv * C::kDV +
                    lane;

@@ -211,3 +211,25 @@ def test_infinite_keys(ctx, hd):
         if dtype != "f32":
             ref, bad = c.exact(), torch.zeros_like(bad)
         check_heads(c.run(ctx), ref, bad, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [MANY, FEW, ALONE])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_scores_of_minus_infinity_throughout(ctx, dtype, hd, shape):
+    """Rows of which every score is -inf: NaN as the softmax of them is (0 is
+    for a sequence without rows); beside a prefix with other scores, nothing."""
+    B, nh, nk, L, lens = shape
+    c = Case(dtype, B, nh, nk, hd, L, lens, seed=hd + 15)
+    c.q.view(B, nh, hd)[..., 2] = 0.5
+    c.k[1, :, 2] = -float("inf")
+    ref, bad = c.exact(), torch.zeros(B, nh, dtype=torch.bool)
+    bad[1, :nh // nk] = L == 0
+    check_heads(c.run(ctx, decay=0.0), ref, bad, dtype)
+    w = c.w[1, 0, :lens[1]]
+    assert bool((w == 0).all() if L else torch.isnan(w).all()), w
+    if L and 0 in lens:
+        b = lens.index(0)
+        c.pk[:, 2] = -float("inf")
+        bad[1, :nh // nk] = bad[b, :nh // nk] = True
+        check_heads(c.run(ctx), c.exact(), bad, dtype)
