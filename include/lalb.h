@@ -235,7 +235,7 @@ LALB_API int lalb_rope_append(lalb_ctx *ctx, const lalb_rope *rope, const lalb_k
  * bits), a query row under a power of two of its own, keys and values under
  * one shared by 16 neighbouring rows (8 at head_dim 256; an element below
  * 2^-17 of the largest there keeps fewer bits); products are summed in fp32.
- * F16 and BF16: weights enter as two parts of that type.  A NaN in a query or
+ * F16 and BF16: weights enter as two parts of that type (22 or 18 bits).  A NaN in a query or
  * a live key makes the heads that read it NaN, in a live value its column of
  * them; so does an infinity in F32, and in F16 and BF16 one in a value (or the
  * column is infinite).  Scores are to stay below 2^23 in size.  A

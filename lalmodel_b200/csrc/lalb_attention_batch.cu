@@ -98,8 +98,8 @@ constexpr int kPad16 = 3, kPadF32 = 2;
 constexpr int kLens = 512;           // sequences whose lengths a CTA keeps in shared memory
 constexpr int kSide = 8;             // tiles whose F32 scales are kept (Cfg checks that they outlive the ring)
 // F32: a stream's tiles between two additions of its O to the sum in memory (1, 2,
-// 4: 41, 37, 31 us for 16 sequences behind 4093 rows, and output errors of 0.9,
-// 1.1 and 1.5e-6 over 1024 rows when parts were still cut off; now 1.1 with 4)
+// 4: 39, 36, 31 us for 16 sequences behind 4093 rows, and output errors of 0.6,
+// 0.7 and 0.9e-6 of the whole)
 constexpr int kFlush = 4;
 constexpr float kShift = 6.0f;       // weights up to 2^6 at the reference maximum, 2^14 before a rescale
 constexpr float kGrow = 8.0f;        // growth of a row's maximum that is left in place
@@ -108,6 +108,7 @@ constexpr int kStageBudget2 = 160 * 1024, kStageBudget1 = 192 * 1024, kStageBudg
 template <class T, int HD>
 struct Cfg {
     static constexpr bool kF32 = sizeof(T) == 4;
+    using H = typename std::conditional<kF32, __half, T>::type;   // the operands' type
     // F32 at head_dim 256: Q's two parts take 256 TMEM columns, so a unit has
     // half of the value columns (the scores are computed for both halves)
     static constexpr int kDV = kF32 && HD == 256 ? 128 : HD;
@@ -384,28 +385,19 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
 }
 
 // x0, x1 as two 16-bit parts each: returns the pair of high parts, lo the
-// rest.  The high part is x cut off (not rounded) to 11 or 8 bits, so that
-// the rest is one mask and one subtraction; with the rest rounded to as many
-// bits again the two are within 2^-22 (fp16) or 2^-16 (bf16) of x.
+// rest.  Both are rounded to nearest, so that the two are within 2^-22 (fp16) or
+// 2^-18 (bf16) of x, and the rests have either sign: F32's product of two
+// rests, which is left out, is 0 on average and not 2^-22 of the whole.
 template <class H>
 __device__ __forceinline__ uint32_t split2(float2 x, uint32_t &lo) {
-    constexpr uint32_t kKeep = std::is_same<H, __half>::value ? 0xffffe000u : 0xffff0000u;
-    const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & kKeep),
-                                 __uint_as_float(__float_as_uint(x.y) & kKeep));
+    const uint32_t hi = pack2<H>(x.x, x.y);
+    float2 h;
+    if constexpr (std::is_same<H, __half>::value)
+        h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    else
+        h = make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
     const float2 r = __fadd2_rn(x, make_float2(-h.x, -h.y));
     lo = pack2<H>(r.x, r.y);
-    if constexpr (std::is_same<H, __half>::value) return pack2<H>(h.x, h.y);
-    return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);   // bf16: the upper halves
-}
-
-// F32: the high part is x rounded to fp16, so that the
-// rests have either sign and the product of two rests, which is left out, is 0
-// on average and not 2^-22 of the whole.
-__device__ __forceinline__ uint32_t split_rn(float2 x, uint32_t &lo) {
-    const uint32_t hi = pack2<__half>(x.x, x.y);
-    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-    const float2 r = __fadd2_rn(x, make_float2(-h.x, -h.y));
-    lo = pack2<__half>(r.x, r.y);
     return hi;
 }
 
@@ -491,8 +483,8 @@ struct RowLoad {
             const int r = r0 + i / kVec * kPer + rr, c = cc + (i % kVec) * 4 * kLanes;
             uint2 hi, lo;
             const float2 a = make_float2(x[i].x * scale, x[i].y * scale), b = make_float2(x[i].z * scale, x[i].w * scale);
-            hi.x = split_rn(a, lo.x);
-            hi.y = split_rn(b, lo.y);
+            hi.x = split2<__half>(a, lo.x);
+            hi.y = split2<__half>(b, lo.y);
             const int unit = (c % W) >> 3;
             const int sw = W == 64 ? unit ^ (r & 7) : unit ^ ((r >> 1) & 3);
             const uint32_t off = (uint32_t)(c / W) * (kTile * W * 2) + r * (W * 2) + sw * 16 + (c & 4) * 2;
@@ -755,8 +747,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
     } else if (warp == C::kSoftWarps) {
         // ================================ MMA ====================================================
         set_regs<C::kSoftRegs ? C::kOtherRegs : 0, false>();
-        constexpr uint32_t kIdS = mma_idesc<typename std::conditional<C::kF32, __half, T>::type>(kTile, false);
-        constexpr uint32_t kIdO = mma_idesc<typename std::conditional<C::kF32, __half, T>::type>(C::kDV, true);
+        constexpr uint32_t kIdS = mma_idesc<typename C::H>(kTile, false);
+        constexpr uint32_t kIdO = mma_idesc<typename C::H>(C::kDV, true);
         constexpr uint32_t kLoK = kTile * HD * 2, kLoV = kTile * C::kDV * 2;
         const uint32_t ring = smem_u32(smem);
         uint32_t tile = 0, segs = 0;        // tiles before the segment: its K(i) is stage 2 (tile + i)
@@ -906,8 +898,8 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                     if constexpr (C::kF32) {
                         const float2 a0 = make_float2(__uint_as_float(x.x) * qs, __uint_as_float(x.y) * qs);
                         const float2 a1 = make_float2(__uint_as_float(x.z) * qs, __uint_as_float(x.w) * qs);
-                        hi[2 * u] = split_rn(a0, lo[2 * u]);
-                        hi[2 * u + 1] = split_rn(a1, lo[2 * u + 1]);
+                        hi[2 * u] = split2<__half>(a0, lo[2 * u]);
+                        hi[2 * u + 1] = split2<__half>(a1, lo[2 * u + 1]);
                     } else {
                         // a negative scale turns the queries' signs
                         const uint32_t f = qs < 0.0f ? 0x80008000u : 0u;
@@ -1325,10 +1317,7 @@ __global__ void __launch_bounds__(Cfg<T, HD>::kThreads, 1)
                                     __ffma2_rn(make_float2(y[j], y[j + 1]), make_float2(f, f), make_float2(e, e));
                                 const float2 p = make_float2(ex2(v.x), ex2(v.y));
                                 sum2 = __fadd2_rn(sum2, p);
-                                if constexpr (C::kF32)
-                                    hi[j >> 1] = split_rn(p, lo[j >> 1]);
-                                else
-                                    hi[j >> 1] = split2<T>(p, lo[j >> 1]);
+                                hi[j >> 1] = split2<typename C::H>(p, lo[j >> 1]);
                             }
                         };
                         if (split) {

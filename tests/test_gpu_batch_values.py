@@ -233,3 +233,23 @@ def test_scores_of_minus_infinity_throughout(ctx, dtype, hd, shape):
         c.pk[:, 2] = -float("inf")
         bad[1, :nh // nk] = bad[b, :nh // nk] = True
         check_heads(c.run(ctx), c.exact(), bad, dtype)
+
+
+def test_bf16_outputs_are_the_nearest(ctx):
+    """How many outputs are not the exact result's nearest bf16.  An error e
+    moves an output x off its nearest with probability e / step(x), steps
+    being 2^-8 to 2^-7 of |x|: 185 e / |x| on average.  Outputs are sums of
+    values of either sign, normal about 0 with deviation s, and an error is of
+    s's size, not of |x|'s: the mean of 1 / |x| over |x| > d is
+    sqrt(2 / pi) (ln(s / d) + 0.06) / s, 6.1 / s for the d = 5e-4 s below which
+    every output is off.  So 185 * 6.1 = 1130 of e / s.  Weights as two rounded
+    bf16 parts are within 2^-18 of a weight, 1.7e-6 on average; scores (8
+    additions cut off at 2^-24 of 4, and the shift's rounding), the
+    exponential (2^-22) and a tile's 8 additions add 1.5e-6 at most:
+    1130 * 3.3e-6 = 3.8e-3.  A first part cut off instead of rounded, within
+    2^-16, is above that: 1130 * 6.8e-6 for the weights alone at their bound,
+    4.3e-3 as measured."""
+    c = Case("bf16", 64, 8, 2, 128, 0, (64,) * 64, seed=77)
+    got, ref = c.run(ctx), c.exact()
+    off = (got != ref.to(torch.bfloat16)).double().mean()
+    assert float(off) <= 3.8e-3, float(off)
