@@ -322,13 +322,19 @@ class KVBatch:
     lalb_kv_batch): k, v CUDA tensors [n_seq][max_ctx][n_kv_head * head_dim]
     (float32, float16 or bfloat16); row_pos int32 and row_weight float32
     [n_seq][n_kv_head][max_ctx], both optional.  The tensors are checked here,
-    once, and stay the cache's."""
+    once, and stay the cache's: calls use the addresses they have now, so the
+    attributes cannot be set anew."""
+
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    row_pos = property(lambda self: self._tensors[2])
+    row_weight = property(lambda self: self._tensors[3])
 
     def __init__(self, k, v, n_kv_head, row_pos=None, row_weight=None):
         if k.dim() != 3 or k.dtype not in _DT or n_kv_head < 1 or k.shape[2] % n_kv_head:
             raise LalbError("KVBatch", -1, "k must be a float32, float16 or bfloat16 tensor "
                                            "[n_seq][max_ctx][n_kv_head * head_dim]")
-        self.k, self.v, self.row_pos, self.row_weight = k, v, row_pos, row_weight
+        self._tensors = k, v, row_pos, row_weight
         self.n_seq, self.max_ctx, self.kvr = k.shape
         self.n_kv_head, self.head_dim = n_kv_head, k.shape[2] // n_kv_head
         self.dtype, self.index = k.dtype, k.get_device()

@@ -52,3 +52,14 @@ def test_batch_python_refusals_need_no_device():
         lb.KVBatch(torch.zeros(2, 4, 64), torch.zeros(2, 4, 64), 1, row_weight=torch.zeros(2, 1, 3))
     with pytest.raises(lb.LalbError):
         lb.Rope(scaling="quadratic")
+
+
+def test_a_cache_keeps_its_tensors():
+    """Calls use the tensors' addresses as they were at first: another tensor in
+    their place would leave calls on memory that is given back."""
+    k = torch.zeros(2, 4, 64)
+    cache = lb.KVBatch(k, k.clone(), 1)
+    assert cache.k is k and cache.row_pos is None
+    for name in ("k", "v", "row_pos", "row_weight"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, torch.zeros(2, 4, 64))
