@@ -171,7 +171,10 @@ LALB_API int lalb_attention_decode(lalb_ctx *ctx, const float *qkv, int n_head, 
  * [max_ctx]): eviction keeps different rows for each KV head, so a row's
  * position is known per head.  Rows may be in any order (their keys are
  * already rotated).  All buffers are device memory of the caller; k and v
- * 16-byte aligned.  head_dim 32, 64, 128 or 256; n_seq*max_ctx <= 2^31 - 256. */
+ * 16-byte aligned.  head_dim 32, 64, 128 or 256; n_seq*max_ctx <= 2^31 - 256.
+ * Attention takes up to 65535 sequences and KV heads, 1024 q heads per KV head
+ * and 2^30 rows of a sequence or a prefix, eviction up to 65535 n_seq*n_kv_head;
+ * more is refused. */
 typedef struct {
     int dtype;               /* LALB_DT_F32, LALB_DT_F16 or LALB_DT_BF16 */
     int n_seq, max_ctx, n_kv_head, head_dim;
@@ -190,7 +193,7 @@ typedef struct {
  *           (turns_fast - turns_slow), 0, 1), f_d (g + (1 - g) / factor);
  *   mscale  multiplies cos and sin.
  * Zero selects a default: rot_dim head_dim, theta 10000, mscale 1.  rot_dim
- * a multiple of 8.  Angles are reduced in double, the rotation is fp32. */
+ * a multiple of 8, theta above 1.  Angles are reduced in double, the rotation is fp32. */
 enum { LALB_ROPE_HALF = 0, LALB_ROPE_INTERLEAVED = 1 };
 enum { LALB_ROPE_UNSCALED = 0, LALB_ROPE_LINEAR = 1, LALB_ROPE_PARTS = 2 };
 typedef struct {
@@ -234,7 +237,8 @@ LALB_API int lalb_rope_append(lalb_ctx *ctx, const lalb_rope *rope, const lalb_k
  * queries, values and weights enter the tensor cores as two fp16 parts (22
  * bits), a query row under a power of two of its own, keys and values under
  * one shared by 16 neighbouring rows (8 at head_dim 256; an element below
- * 2^-17 of the largest there keeps fewer bits); products are summed in fp32.
+ * 2^-17 of the largest there, or below 2^-77, keeps fewer bits); products are
+ * summed in fp32.
  * F16 and BF16: weights enter as two parts of that type (22 or 18 bits).  A NaN in a query or
  * a live key makes the heads that read it NaN, in a live value its column of
  * them; so does an infinity in F32, and in F16 and BF16 one in a value (or the

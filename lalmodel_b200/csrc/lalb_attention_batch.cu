@@ -61,18 +61,21 @@
 //
 // What bounds it (B200; bytes and products that it cannot do without against the
 // measured 6540 GB/s and 1637 TFLOP/s; a pass from a graph, caches warm):
-//   64 sequences, 16384 + 0..1000 bf16 rows, 28 heads on 4 of 128: 52 us; the
+//   64 sequences, 16384 + 0..1000 bf16 rows, 28 heads on 4 of 128: 53 us; the
 //     memory floor is 15 us, the tensor floor (three products' time for two)
-//     14; tiles come from L2 at 6.4 TB/s, 32 KB for 128 query rows, as fast
-//     as the softmax warps weigh them (0.9 us a tile), and the ends of some 400
-//     segments cost 3 us each;
+//     14; nothing is full (tensor pipe 45 %, issue slots 25 %, DRAM 25 %, L2
+//     19 %): a tile takes its CTA 0.9 us, a chain of scores, maximum, exponentials,
+//     parts and hand-over that the two streams overlap only in part, and the ends
+//     of some 400 segments cost 3 us each;
 //   16 sequences, 4093 + 1..700 F32 rows: 31 us, floor 6; one tile takes its
-//     CTA 2 us, most of it in the loaders' splitting and the softmax's waits;
-//   5 sequences, 333 + 100..2000 F32 rows at head_dim 256: 44 us, floor 7; one
+//     CTA 2 us, most of it in the loaders' splitting and the softmax's waits
+//     (tensor pipe 17 %, DRAM 18 %, instruction cache hits 81 %);
+//   5 sequences, 333 + 100..2000 F32 rows at head_dim 256: 46 us, floor 7; one
 //     softmax stream for half of the value columns, 64 KB of keys split for each,
 //     and 8 us a segment to bring Q's two parts into TMEM;
-//   8 sequences, 3001..8191 f16 rows, 16 heads on 8 of 64: 40 us, floor 14;
-//   one sequence of 812 F32 rows: 16 us, of which each CTA's single tile takes 8
+//   8 sequences, 3001..8191 f16 rows, 16 heads on 8 of 64: 39 us, floor 14; the
+//     same chain, of which 2 of 32 lanes hold a query row;
+//   one sequence of 812 F32 rows: 17 us, of which each CTA's single tile takes 8
 //     from launch to partial, all latency: lengths, Q, rows, S, weights, PV in turn.
 //
 // TMEM columns: S/P buffers from 0, then Q, O up to 511.  Every wait is bounded.
@@ -322,6 +325,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, unsign
     return __all_sync(0xffffffffu, wait_bounded(bar, parity, status));
 }
 
+// 2^x within 2^-22 of it, 0 below 2^-126.
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
